@@ -26,6 +26,9 @@ BUILD = os.path.join(PKG, '..', 'build', 'raft_amd')
 OUT = os.path.join(PKG, '_C.so')
 OUT_CPU = os.path.join(PKG, '_cpu.so')
 ARCH = os.environ.get('RAFT_AMD_ARCH', 'gfx950')
+# device code without the packed fp32 instructions (v_pk_add / mul / fma_f32): -O3 forms them from
+# ordinary float code, and some of their operand forms have given wrong sums on gfx950 now and then
+NO_PACKED_FP32 = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 
 
@@ -72,7 +75,7 @@ def build(force=False, jobs=None, verbose=False):
     # ---- GPU extension
     kernels = sorted(glob.glob(os.path.join(CSRC, 'kernels', '*.hip')))
     common = ['-O3', '-fPIC', '-std=c++17', '--offload-arch=%s' % ARCH, '-D__HIP_PLATFORM_AMD__=1',
-              '-ffp-contract=fast', '-Wno-unused-result']
+              '-ffp-contract=fast', '-Wno-unused-result'] + NO_PACKED_FP32
     jobs_list = []
     objs = []
     for src in kernels:

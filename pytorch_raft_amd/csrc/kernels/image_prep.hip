@@ -37,9 +37,13 @@ __global__ __launch_bounds__(256) void image_prep_kernel(const float* __restrict
     const float* src = n < B ? a + n * 3 * HW : b + (n - B) * 3 * HW;
 #pragma unroll
     for (int c = 0; c < 3; ++c) {
+      // each step rounded to fp32 by itself: left to the compiler, the difference and the conversion
+      // to fp16 become one mixed-precision instruction with a single rounding
       float t = src[c * HW + s] * inv255;
+      asm volatile("" : "+v"(t));
       t = 2.0f * t;
       t = t - 1.0f;
+      asm volatile("" : "+v"(t));
       put<OT>(out, p * 3 + c, t);
     }
   }
