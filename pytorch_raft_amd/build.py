@@ -4,7 +4,7 @@
 
 * every ``csrc/kernels/*.hip`` is compiled by ``hipcc --offload-arch=gfx950 -O3`` WITHOUT torch
   headers (plain HIP, seconds per file);
-* ``csrc/bindings.cpp`` (TORCH_LIBRARY registration) is compiled against the installed torch;
+* ``csrc/bindings*.cpp`` (TORCH_LIBRARY registration) are compiled against the installed torch;
 * everything is linked into one shared object next to this file, so it travels with the repo
   snapshot to the GPU box and is what ``torch.ops.load_library`` loads at import time.
 
@@ -59,7 +59,7 @@ def _up_to_date():
     """Both libraries newer than every source / header: nothing to do (object files not needed,
     so the build/ directory does not have to travel with the tree)."""
     headers = glob.glob(os.path.join(CSRC, '**', '*.h'), recursive=True)
-    gpu_srcs = glob.glob(os.path.join(CSRC, 'kernels', '*.hip')) + [os.path.join(CSRC, 'bindings.cpp')]
+    gpu_srcs = glob.glob(os.path.join(CSRC, 'kernels', '*.hip')) + glob.glob(os.path.join(CSRC, 'bindings*.cpp'))
     cpu_srcs = glob.glob(os.path.join(CSRC, 'cpu', '*.cpp'))
     return not _newer(OUT, gpu_srcs + headers) and not _newer(OUT_CPU, cpu_srcs + headers)
 
@@ -83,10 +83,11 @@ def build(force=False, jobs=None, verbose=False):
         objs.append(obj)
         if force or _newer(obj, [src] + headers):
             jobs_list.append([HIPCC] + common + ['-c', src, '-o', obj])
-    bsrc = os.path.join(CSRC, 'bindings.cpp')
-    bobj = os.path.join(BUILD, 'bindings.o')
-    objs.append(bobj)
-    if force or _newer(bobj, [bsrc] + headers):
+    for bsrc in sorted(glob.glob(os.path.join(CSRC, 'bindings*.cpp'))):
+        bobj = os.path.join(BUILD, os.path.splitext(os.path.basename(bsrc))[0] + '.o')
+        objs.append(bobj)
+        if not (force or _newer(bobj, [bsrc] + headers)):
+            continue
         flags = ['-O2', '-fPIC', '-std=c++17', '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1',
                  '-DHIPBLAS_V2', '-D_GLIBCXX_USE_CXX11_ABI=%d' % abi, '-Wno-unused-result',
                  '-Wno-deprecated-declarations']

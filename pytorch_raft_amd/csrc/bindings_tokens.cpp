@@ -1,0 +1,180 @@
+// Torch registration of the token operators: attention (forward, backward), root-mean-square norm
+// (forward, backward, 8-bit output), 8-bit integer product.  Same rules as bindings.cpp: every
+// argument is checked on the host before a launch, kernels run on the current stream of the tensors'
+// device, outputs and workspaces come from torch's allocator.
+#include <torch/library.h>
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+
+#include <cmath>
+#include <limits>
+#include <vector>
+
+#include "kernels/launchers.h"
+
+namespace {
+
+using at::Tensor;
+typedef const std::optional<Tensor>& OptTensor;
+
+hipStream_t cur_stream() { return c10::hip::getCurrentHIPStream().stream(); }
+
+bool given(OptTensor t) { return t.has_value() && t->defined(); }
+
+int dtype_code(const Tensor& t, const char* name) {
+  const auto st = t.scalar_type();
+  TORCH_CHECK(st == at::kBFloat16 || st == at::kHalf || st == at::kFloat, name,
+              " must be bfloat16, float16 or float32, got ", st);
+  return st == at::kBFloat16 ? 0 : (st == at::kHalf ? 1 : 2);
+}
+
+// (B, L, heads, D) whose rows the kernels can read in 16-byte pieces; anything else is copied once
+Tensor token_rows(const Tensor& t) {
+  const int64_t es = t.element_size();
+  bool ok = t.stride(3) == 1 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
+  int64_t reach = 0;
+  for (int d = 0; d < 3; ++d) {
+    if (t.size(d) == 1) continue;
+    ok = ok && t.stride(d) * es % 16 == 0 && t.stride(d) >= t.size(3);
+    if (d > 0) reach += t.stride(d) * es * std::min<int64_t>(t.size(d), 72);
+  }
+  ok = ok && reach < (int64_t(1) << 30);  // a tile's rows lie within a descriptor's 32-bit offsets
+  // (.contiguous() alone would keep a dense tensor that starts off 16 bytes)
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+// stride of a dimension of size 1 is never used: 0 keeps offsets small
+int64_t stride_of(const Tensor& t, int d) { return t.size(d) == 1 ? 0 : t.stride(d); }
+
+void check_ints(OptTensor t, const Tensor& like, int64_t n, const char* name) {
+  if (!given(t)) return;
+  TORCH_CHECK(t->device() == like.device() && t->scalar_type() == at::kInt && t->dim() == 1 &&
+                  t->size(0) == n && t->is_contiguous(),
+              name, " must be a contiguous int32 tensor of shape (", n, ",) on the device of q");
+}
+
+AttnArgs attn_args(const Tensor& q, const Tensor& k, const Tensor& v, double scale, bool causal,
+                   OptTensor mask, OptTensor lengths, OptTensor q_offset) {
+  TORCH_CHECK(q.is_cuda() && k.device() == q.device() && v.device() == q.device(),
+              "q, k and v must be on one GPU");
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.sizes() == k.sizes(),
+              "q must be (B, Lq, H, D), k and v (B, Lk, Hkv, D)");
+  TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(),
+              "q, k and v must have one dtype");
+  TORCH_CHECK(k.size(0) == q.size(0) && k.size(3) == q.size(3), "q and k disagree on batch or head size");
+  TORCH_CHECK(k.size(2) > 0 && q.size(2) > 0 && q.size(2) % k.size(2) == 0,
+              "the query heads must be a multiple of the key heads");
+  const int64_t B = q.size(0), Lq = q.size(1), H = q.size(2), D = q.size(3), Lk = k.size(1);
+  TORCH_CHECK(D >= 8 && D <= 128 && D % 8 == 0, "head size must be a multiple of 8 up to 128, got ", D);
+  TORCH_CHECK(std::isfinite(scale) && scale > 0, "scale must be positive and finite");
+  const int64_t big = int64_t(1) << 26;
+  TORCH_CHECK(B * H * std::max<int64_t>(Lq, 1) < big && B * k.size(2) * std::max<int64_t>(Lk, 1) < big * 16 && Lk < big * 16,
+              "attention: too many rows for one call");
+  AttnArgs a = {};
+  a.dtype = dtype_code(q, "q");
+  a.B = (int)B;
+  a.Lq = (int)Lq;
+  a.Lk = (int)Lk;
+  a.Hkv = (int)k.size(2);
+  a.G = (int)(H / k.size(2));
+  a.D = (int)D;
+  a.DP = (int)((D + 31) / 32 * 32);
+  a.scale = (float)scale;
+  a.scale_log2 = (float)(scale * 1.4426950408889634);
+  a.causal = causal;
+  a.q = q.data_ptr();
+  a.q_sb = stride_of(q, 0), a.q_sl = stride_of(q, 1), a.q_sh = stride_of(q, 2);
+  a.k = k.data_ptr();
+  a.k_sb = stride_of(k, 0), a.k_sl = stride_of(k, 1), a.k_sh = stride_of(k, 2);
+  a.v = v.data_ptr();
+  a.v_sb = stride_of(v, 0), a.v_sl = stride_of(v, 1), a.v_sh = stride_of(v, 2);
+  check_ints(lengths, q, B, "lengths");
+  check_ints(q_offset, q, B, "q_offset");
+  a.lengths = given(lengths) ? lengths->data_ptr<int>() : nullptr;
+  a.q_offset = given(q_offset) ? q_offset->data_ptr<int>() : nullptr;
+  a.nsplit = 1;
+  if (given(mask)) {
+    const Tensor& m = *mask;
+    TORCH_CHECK(m.device() == q.device() && m.scalar_type() == at::kBool && m.dim() == 4 && m.size(0) == B &&
+                    m.size(1) == H && m.size(2) == Lq && m.size(3) == Lk,
+                "mask must be a bool tensor expanded to (B, H, Lq, Lk) on the device of q");
+    a.mask = reinterpret_cast<const uint8_t*>(m.data_ptr());
+    a.m_sb = stride_of(m, 0), a.m_sh = stride_of(m, 1), a.m_sq = stride_of(m, 2), a.m_sk = stride_of(m, 3);
+    a.mask_mode = a.m_sh == 0 && a.m_sq == 0 ? 1 : 2;
+  }
+  return a;
+}
+
+// -> {out (B, Lq, H, D), log2-sum-exp2 of the rows (B, Hkv, Lq * G) or empty}
+std::vector<Tensor> attn_fwd(const Tensor& q0, const Tensor& k0, const Tensor& v0, double scale, bool causal,
+                             OptTensor mask, OptTensor lengths, OptTensor q_offset, bool need_lse) {
+  TORCH_CHECK(q0.dim() == 4 && k0.dim() == 4 && v0.dim() == 4, "q must be (B, Lq, H, D), k and v (B, Lk, Hkv, D)");
+  c10::DeviceGuard g(q0.device());
+  const Tensor q = token_rows(q0), k = token_rows(k0), v = token_rows(v0);
+  AttnArgs a = attn_args(q, k, v, scale, causal, mask, lengths, q_offset);
+  const auto f32 = q.options().dtype(at::kFloat);
+  const int64_t R = (int64_t)a.G * a.Lq;
+  if (a.B == 0 || a.Lq == 0 || a.Lk == 0)
+    return {at::zeros(q.sizes(), q.options()),
+            need_lse ? at::full({a.B, a.Hkv, R}, std::numeric_limits<float>::infinity(), f32) : at::empty({0}, f32)};
+  Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  Tensor lse = need_lse ? at::empty({a.B, a.Hkv, R}, f32) : at::empty({0}, f32);
+  a.o = out.data_ptr();
+  a.lse = need_lse ? lse.data_ptr<float>() : nullptr;
+  a.nsplit = attn_splits(a);
+  Tensor part;
+  if (a.nsplit > 1) {
+    const int64_t n = (int64_t)a.B * a.Hkv * a.nsplit * R;
+    part = at::empty({n * (a.DP + 2)}, f32);
+    a.part = part.data_ptr<float>();
+    a.part_ml = a.part + n * a.DP;
+  }
+  launch_attn_fwd(a, cur_stream());
+  return {out, lse};
+}
+
+// -> {dq, dk, dv}, contiguous
+std::vector<Tensor> attn_bwd(const Tensor& dout0, const Tensor& q0, const Tensor& k0, const Tensor& v0,
+                             const Tensor& out, const Tensor& lse, double scale, bool causal, OptTensor mask,
+                             OptTensor lengths, OptTensor q_offset) {
+  TORCH_CHECK(q0.dim() == 4 && k0.dim() == 4 && v0.dim() == 4, "q must be (B, Lq, H, D), k and v (B, Lk, Hkv, D)");
+  c10::DeviceGuard g(q0.device());
+  TORCH_CHECK(dout0.device() == q0.device() && dout0.scalar_type() == q0.scalar_type() && dout0.sizes() == q0.sizes(),
+              "dout must match q");
+  const Tensor q = token_rows(q0), k = token_rows(k0), v = token_rows(v0), dout = token_rows(dout0);
+  AttnArgs a = attn_args(q, k, v, scale, causal, mask, lengths, q_offset);
+  const int64_t R = (int64_t)a.G * a.Lq;
+  TORCH_CHECK(out.device() == q.device() && out.scalar_type() == q.scalar_type() && out.sizes() == q.sizes() && out.is_contiguous(),
+              "out must be the forward's");
+  TORCH_CHECK(lse.device() == q.device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() && lse.numel() == (int64_t)a.B * a.Hkv * R,
+              "lse must be the forward's");
+  Tensor dq = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  Tensor dk = at::empty(k.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  Tensor dv = at::empty(k.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  if (a.B == 0 || a.Lq == 0 || a.Lk == 0) return {dq.zero_(), dk.zero_(), dv.zero_()};
+  Tensor ws = at::empty({(int64_t)a.B * a.Hkv * R + 2}, q.options().dtype(at::kFloat));
+  a.o = out.data_ptr();
+  a.lse = lse.data_ptr<float>();
+  a.dout = dout.data_ptr();
+  a.d_sb = stride_of(dout, 0), a.d_sl = stride_of(dout, 1), a.d_sh = stride_of(dout, 2);
+  a.delta = ws.data_ptr<float>();
+  a.amax = reinterpret_cast<uint32_t*>(a.delta + (int64_t)a.B * a.Hkv * R);
+  a.dq = dq.data_ptr();
+  a.dk = dk.data_ptr();
+  a.dv = dv.data_ptr();
+  launch_attn_bwd(a, cur_stream());
+  return {dq, dk, dv};
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(raft_amd, m) {
+  m.def("attn_fwd(Tensor q, Tensor k, Tensor v, float scale, bool causal, Tensor? mask, Tensor? lengths, Tensor? q_offset, bool need_lse) -> Tensor[]");
+  m.def("attn_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, float scale, bool causal, Tensor? mask, Tensor? lengths, Tensor? q_offset) -> Tensor[]");
+}
+
+TORCH_LIBRARY_IMPL(raft_amd, CUDA, m) {
+  m.impl("attn_fwd", &attn_fwd);
+  m.impl("attn_bwd", &attn_bwd);
+}

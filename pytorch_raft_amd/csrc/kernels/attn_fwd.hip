@@ -1,0 +1,453 @@
+// Softmax attention over tokens, forward: o_i = sum_j softmax_j(scale q_i . k_j) v_j.
+//
+// One pass over the keys with a running maximum and sum.  A wave owns 32 rows (queries); the scores
+// of a key block are computed transposed, S^T = K Q^T, so that a lane holds one query's scores:
+// maximum and sum are register reductions plus one half-wave exchange, rescaling the output is one
+// multiply per register, and the probabilities are the B operand of O^T = V^T P^T as they lie.
+#include "attn_common.h"
+
+namespace attn_detail {
+
+template <typename T, int DP>
+struct FwdCfg {
+  static constexpr int BK = sizeof(T) == 4 ? 32 : 64;  // keys per tile
+  static constexpr int NW = 4, NT = 256, BM = 32 * NW;
+  static constexpr int TILE = BK * DP * (int)sizeof(T);
+};
+
+// Running softmax state of a wave's 32 rows (one per lane pair) and the output accumulators.
+template <typename T, int DP>
+struct RowState {
+  using TL = Tile<T, DP>;
+  using Frag = typename TL::Frag;
+  static constexpr int DB = DP / 32, DT = DP / 16;
+  Frag q[DT];
+  f32x16 o[DB];
+  float m, l;  // reference exponent (log2 units), this half-wave's part of the sum
+
+  __device__ __forceinline__ void init() {
+#pragma unroll
+    for (int i = 0; i < DB; ++i) o[i] = zero16();
+    m = -INFINITY;
+    l = 0.f;
+  }
+  // query row from global memory (zeros past the last row and past D)
+  __device__ __forceinline__ void load_q(const T* p, bool ok, int D, int hi) {
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+      const int d = 16 * t + 8 * hi;
+      Frag f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = (T)0.f;
+      if (ok && d < D) f = *reinterpret_cast<const Frag*>(p + d);
+      q[t] = f;
+    }
+  }
+  // scores of NB blocks of 32 keys
+  template <int NB>
+  __device__ __forceinline__ void scores(const uint8_t* kt, f32x16 (&s)[NB], int lane) const {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) s[b] = zero16();
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+        s[b] = mma(TL::rows(kt, b * 32 + (lane & 31), t, lane >> 5), q[t], s[b]);
+  }
+  // scores -> probabilities relative to the running reference, which moves (rescaling the output)
+  // only when a row's maximum has outgrown it by 2^8: the result is the same, since sum and
+  // output carry the same factor, and p <= 2^8 is far from every type's limit.
+  template <int NB>
+  __device__ __forceinline__ void softmax(f32x16 (&s)[NB], float c) {
+    float mx = s[0][0];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
+    mx = fmaxf(mx, other_half(mx)) * c;
+    if (__any(mx > m + 8.f)) {
+      const float mn = fmaxf(m, mx);
+      const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= al;
+#pragma unroll
+      for (int i = 0; i < DB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[i][r] *= al;
+    }
+    const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[b][r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], c, -ms));
+        l += s[b][r];
+      }
+  }
+  template <int NB>
+  __device__ __forceinline__ void values(const uint8_t* vt, const f32x16 (&s)[NB], int lane) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const Frag p = to_frag<T>(s[b], t);
+#pragma unroll
+        for (int i = 0; i < DB; ++i) o[i] = mma(TL::cols(vt, b * 32 + 16 * t, i, lane), p, o[i]);
+      }
+  }
+};
+
+// keys at or past `lim` (this lane's row) and keys hidden by the mask -> -inf.  bias: per-key 0 / -inf
+// of a key mask (LDS); full: this row's bytes of a (query, key) mask at the tile's first key.
+template <int NB, int MASK>
+__device__ __forceinline__ void hide(f32x16 (&s)[NB], int left, int hi, const float* bias, const uint8_t* full,
+                                     int64_t msk, int nkeys) {
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int j = b * 32 + (r >> 2) * 8 + hi * 4 + (r & 3);
+      float v = s[b][r];
+      if constexpr (MASK == 1) v += bias[j];
+      bool see = j < left;
+      if constexpr (MASK == 2) see = see && j < nkeys && full[min(j, nkeys - 1) * msk] != 0;
+      s[b][r] = see ? v : -INFINITY;
+    }
+}
+
+// lane's output row (column of O^T): 4 consecutive channels per 4 registers
+template <typename T, int DB>
+__device__ __forceinline__ void store_row(T* p, const f32x16 (&o)[DB], float f, int D, int hi) {
+#pragma unroll
+  for (int i = 0; i < DB; ++i)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = i * 32 + g * 8 + hi * 4;
+      if (d < D) {
+        typedef T v4 __attribute__((ext_vector_type(4)));
+        v4 w;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = (T)(o[i][4 * g + k] * f);
+        *reinterpret_cast<v4*>(p + d) = w;
+      }
+    }
+}
+
+template <typename T, int DP, int MASK>
+__global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
+  using C = FwdCfg<T, DP>;
+  using TL = Tile<T, DP>;
+  constexpr int BK = C::BK, NB = BK / 32;
+  __shared__ __attribute__((aligned(16))) uint8_t kv[2][2][C::TILE];
+  __shared__ __attribute__((aligned(16))) float bias[2][BK];
+
+  const int R = a.G * a.Lq;
+  const int tiles = (R + C::BM - 1) / C::BM;
+  const int id = xcd_order(blockIdx.x, gridDim.x);
+  if (id >= tiles * a.nsplit * a.B * a.Hkv) return;
+  const int tile = tiles - 1 - id % tiles, split = id / tiles % a.nsplit, bh = id / tiles / a.nsplit;
+  const int b = bh / a.Hkv, hk = bh - b * a.Hkv;
+  const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r0 = tile * C::BM + wave * 32, row = r0 + (lane & 31);
+  const bool ok = row < R;
+  const int qi = min(row, R - 1) / a.G, g = min(row, R - 1) - qi * a.G;
+  const int h = hk * a.G + g;
+
+  const int len = item_len(a, b), off = item_off(a, b);
+  const int lim = a.causal ? max(0, min(len, off + qi + 1)) : len;     // keys this lane's row sees
+  const int wlim = !a.causal ? len : max(0, min(len, off + (min(r0 + 31, R - 1)) / a.G + 1));
+  const int wmin = !a.causal ? len : max(0, min(len, off + min(r0, R - 1) / a.G + 1));
+  const int blim = !a.causal ? len : max(0, min(len, off + (min(tile * C::BM + C::BM, R) - 1) / a.G + 1));
+  int t0 = 0, t1 = (blim + BK - 1) / BK;
+  if (a.nsplit > 1) {
+    const int per = ((a.Lk + BK - 1) / BK + a.nsplit - 1) / a.nsplit;
+    t0 = min(t1, split * per);
+    t1 = min(t1, t0 + per);
+  }
+
+  RowState<T, DP> st;
+  st.init();
+  st.load_q(reinterpret_cast<const T*>(a.q) + b * a.q_sb + (int64_t)qi * a.q_sl + h * a.q_sh, ok, a.D, hi);
+
+  const uint32_t kp = (uint32_t)(a.k_sl * TL::ES), vp = (uint32_t)(a.v_sl * TL::ES);
+  const uint8_t* kb = reinterpret_cast<const uint8_t*>(a.k) + (b * a.k_sb + hk * a.k_sh) * TL::ES;
+  const uint8_t* vb = reinterpret_cast<const uint8_t*>(a.v) + (b * a.v_sb + hk * a.v_sh) * TL::ES;
+  Loader<T, DP, BK, 256> lk, lv;
+  lk.init(tid, kp, a.D * TL::ES);
+  lv.init(tid, vp, a.D * TL::ES);
+  const uint32_t lds = raft_lds_addr(&kv[0][0][0]) + wave * 1024;
+  const uint8_t* mk = MASK ? a.mask + b * a.m_sb + (MASK == 2 ? h * a.m_sh + (int64_t)qi * a.m_sq : 0) : nullptr;
+
+  auto issue = [&](int t, int buf) {
+    const int k0 = t * BK, n = min(BK, len - k0);
+    const rsrc_t rk = rows_rsrc(kb + (int64_t)k0 * kp, n, kp, a.D * TL::ES);
+    const rsrc_t rv = rows_rsrc(vb + (int64_t)k0 * vp, n, vp, a.D * TL::ES);
+    if constexpr (MASK == 1) {
+      // a hidden key's row is not fetched at all (zeros), whatever it holds
+      using L = Loader<T, DP, BK, 256>;
+#pragma unroll
+      for (int j = 0; j < L::PER; ++j) {
+        const int r = L::row_of(tid, j);
+        const bool see = r < n && mk[(int64_t)(k0 + min(r, n - 1)) * a.m_sk] != 0;
+        raft_dma16(rk, lds + (2 * buf) * C::TILE + j * 4096, see ? lk.off[j] : kOob);
+        raft_dma16(rv, lds + (2 * buf + 1) * C::TILE + j * 4096, see ? lv.off[j] : kOob);
+      }
+      if (tid < BK) bias[buf][tid] = tid < n && mk[(int64_t)(k0 + min(tid, n - 1)) * a.m_sk] != 0 ? 0.f : -INFINITY;
+    } else {
+      lk.issue(rk, lds + (2 * buf) * C::TILE);
+      lv.issue(rv, lds + (2 * buf + 1) * C::TILE);
+    }
+  };
+
+  if (t0 < t1) issue(t0, 0);
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1, k0 = t * BK;
+    raft_wait_vmcnt<0>();
+    __syncthreads();  // tile t has landed for all waves, and all have left tile t - 1's buffer
+    if (t + 1 < t1) issue(t + 1, buf ^ 1);
+    if (k0 < wlim) {
+      f32x16 s[NB];
+      st.scores(&kv[buf][0][0], s, lane);
+      if (MASK || k0 + BK > wmin)
+        hide<NB, MASK>(s, lim - k0, hi, bias[buf], MASK == 2 ? mk + (int64_t)k0 * a.m_sk : nullptr, a.m_sk, a.Lk - k0);
+      st.softmax(s, a.scale_log2);
+      st.values(&kv[buf][1][0], s, lane);
+    }
+  }
+
+  const float l = st.l + other_half(st.l);
+  if (!ok) return;
+  if (a.nsplit > 1) {
+    const int64_t p = ((int64_t)bh * a.nsplit + split) * R + row;
+    store_row<float>(a.part + p * DP, st.o, 1.f, DP, hi);
+    if (hi == 0) {
+      a.part_ml[2 * p] = st.m;
+      a.part_ml[2 * p + 1] = l;
+    }
+    return;
+  }
+  store_row<T>(reinterpret_cast<T*>(a.o) + (((int64_t)b * a.Lq + qi) * a.Hkv * a.G + h) * a.D, st.o,
+               l > 0.f || l != l ? 1.f / l : 0.f, a.D, hi);
+  if (a.lse && hi == 0) a.lse[(int64_t)bh * R + row] = l > 0.f || l != l ? st.m + log2f(l) : INFINITY;
+}
+
+// ---- few rows (R <= 32) over long keys: bound by reading K and V once.  The four waves of a
+// workgroup take different 32-key blocks of the workgroup's key range, each through LDS buffers of
+// its own (no barrier in the loop), and are joined in LDS at the end.
+template <typename T, int DP, int MASK>
+__global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnArgs a) {
+  using TL = Tile<T, DP>;
+  constexpr int TILE = 32 * DP * (int)sizeof(T);
+  constexpr int DB = DP / 32;
+  // two buffers of K and V for each wave where they fit the 160 KB (fp32 heads over 64: one)
+  constexpr int BUFS = 4 * 2 * 2 * TILE <= 128 * 1024 ? 2 : 1;
+  constexpr int BUF = 4 * 2 * BUFS * TILE, JOIN = 4 * 32 * (DP + 4) * 4;
+  __shared__ __attribute__((aligned(16))) uint8_t sm[BUF > JOIN ? BUF : JOIN];
+  __shared__ float ml[4][32][2];
+
+  const int R = a.G * a.Lq;
+  const int id = xcd_order(blockIdx.x, gridDim.x);
+  if (id >= a.nsplit * a.B * a.Hkv) return;
+  const int split = id % a.nsplit, bh = id / a.nsplit;
+  const int b = bh / a.Hkv, hk = bh - b * a.Hkv;
+  const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int row = lane & 31;
+  const bool ok = row < R;
+  const int qi = min(row, R - 1) / a.G, g = min(row, R - 1) - qi * a.G, h = hk * a.G + g;
+  const int len = item_len(a, b), off = item_off(a, b);
+  const int lim = a.causal ? max(0, min(len, off + qi + 1)) : len;
+  const int wmin = !a.causal ? len : max(0, min(len, off + 1));
+  const int blim = !a.causal ? len : max(0, min(len, off + a.Lq));
+  // the item's own blocks are dealt evenly over the splits
+  const int blocks = (blim + 31) / 32;
+  const int per = (blocks + a.nsplit - 1) / a.nsplit;
+  const int t0 = min(blocks, split * per), t1 = min(blocks, t0 + per);
+
+  RowState<T, DP> st;
+  st.init();
+  st.load_q(reinterpret_cast<const T*>(a.q) + b * a.q_sb + (int64_t)qi * a.q_sl + h * a.q_sh, ok, a.D, hi);
+  const uint32_t kp = (uint32_t)(a.k_sl * TL::ES), vp = (uint32_t)(a.v_sl * TL::ES);
+  const uint8_t* kb = reinterpret_cast<const uint8_t*>(a.k) + (b * a.k_sb + hk * a.k_sh) * TL::ES;
+  const uint8_t* vb = reinterpret_cast<const uint8_t*>(a.v) + (b * a.v_sb + hk * a.v_sh) * TL::ES;
+  using L = Loader<T, DP, 32, 64>;
+  L lk, lv;
+  lk.init(lane, kp, a.D * TL::ES);
+  lv.init(lane, vp, a.D * TL::ES);
+  uint8_t* mine = sm + wave * 2 * BUFS * TILE;
+  const uint32_t lds = raft_lds_addr(sm) + wave * 2 * BUFS * TILE;
+  const uint8_t* mk = MASK ? a.mask + b * a.m_sb + (MASK == 2 ? h * a.m_sh + (int64_t)qi * a.m_sq : 0) : nullptr;
+
+  auto issue = [&](int t, int buf) {
+    const int k0 = t * 32, n = min(32, len - k0);
+    const rsrc_t rk = rows_rsrc(kb + (int64_t)k0 * kp, n, kp, a.D * TL::ES);
+    const rsrc_t rv = rows_rsrc(vb + (int64_t)k0 * vp, n, vp, a.D * TL::ES);
+    if constexpr (MASK == 1) {
+#pragma unroll
+      for (int j = 0; j < L::PER; ++j) {
+        const int r = L::row_of(lane, j);
+        const bool see = r < n && mk[(int64_t)(k0 + min(r, n - 1)) * a.m_sk] != 0;
+        raft_dma16(rk, lds + (2 * buf) * TILE + j * 1024, see ? lk.off[j] : kOob);
+        raft_dma16(rv, lds + (2 * buf + 1) * TILE + j * 1024, see ? lv.off[j] : kOob);
+      }
+    } else {
+      lk.issue(rk, lds + (2 * buf) * TILE);
+      lv.issue(rv, lds + (2 * buf + 1) * TILE);
+    }
+  };
+
+  int t = t0 + wave;
+  if (BUFS == 2 && t < t1) issue(t, 0);
+  for (int buf = 0; t < t1; t += 4, buf ^= BUFS - 1) {
+    const int k0 = t * 32;
+    // the next block's DMA overwrites the buffer read two blocks ago: those reads have returned
+    // (their products were issued), and the wait below leaves only the next block in flight
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    if (BUFS == 1) {
+      issue(t, 0);
+      raft_wait_vmcnt<0>();
+    } else if (t + 4 < t1) {
+      issue(t + 4, buf ^ 1);
+      raft_wait_vmcnt<2 * L::PER>();
+    } else {
+      raft_wait_vmcnt<0>();
+    }
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
+    f32x16 s[1];
+    st.scores(mine + (2 * buf) * TILE, s, lane);
+    if (MASK || k0 + 32 > wmin) {
+      if constexpr (MASK == 1) {
+        const int64_t left = len - 1 - k0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = (r >> 2) * 8 + hi * 4 + (r & 3);
+          const bool see = j < lim - k0 && mk[(k0 + (j < left ? j : left)) * a.m_sk] != 0;
+          s[0][r] = see ? s[0][r] : -INFINITY;
+        }
+      } else {
+        hide<1, MASK>(s, lim - k0, hi, nullptr, MASK == 2 ? mk + (int64_t)k0 * a.m_sk : nullptr, a.m_sk, a.Lk - k0);
+      }
+    }
+    st.softmax(s, a.scale_log2);
+    st.values(mine + (2 * buf + 1) * TILE, s, lane);
+    asm volatile("" ::: "memory");
+  }
+
+  // join the waves: common reference exponent, then sums over waves of the scaled outputs
+  const float l = st.l + other_half(st.l);
+  if (hi == 0) {
+    ml[wave][row][0] = st.m;
+    ml[wave][row][1] = l;
+  }
+  __syncthreads();  // also: every wave has left its tiles, which the outputs now overwrite
+  float mt = -INFINITY, lt = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) mt = fmaxf(mt, ml[w][row][0]);
+  const float ms = mt == -INFINITY ? 0.f : mt;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) lt += ml[w][row][1] * __builtin_amdgcn_exp2f(ml[w][row][0] - ms);
+  const float f = __builtin_amdgcn_exp2f(st.m - ms);
+  float* jo = reinterpret_cast<float*>(sm);
+  store_row<float>(jo + (wave * 32 + row) * (DP + 4), st.o, f, DP, hi);
+  __syncthreads();
+  const bool some = lt > 0.f || lt != lt;
+  if (a.nsplit == 1 && a.lse && wave == 0 && hi == 0 && ok) a.lse[(int64_t)bh * R + row] = some ? mt + log2f(lt) : INFINITY;
+  if (a.nsplit > 1 && wave == 0 && hi == 0 && ok) {
+    const int64_t p = ((int64_t)bh * a.nsplit + split) * R + row;
+    a.part_ml[2 * p] = mt;
+    a.part_ml[2 * p + 1] = lt;
+  }
+  // thread -> (row, channel): rows of DP channels
+  if (wave == 0 && hi == 0) ml[0][row][0] = some ? 1.f / lt : 0.f;  // read after the barrier below
+  __syncthreads();
+  for (int e = tid; e < R * DP; e += 256) {
+    const int r = e / DP, d = e - r * DP;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) v += jo[(w * 32 + r) * (DP + 4) + d];
+    if (a.nsplit > 1) {
+      a.part[(((int64_t)bh * a.nsplit + split) * R + r) * DP + d] = v;
+    } else if (d < a.D) {
+      const int q2 = r / a.G, g2 = r - q2 * a.G;
+      reinterpret_cast<T*>(a.o)[(((int64_t)b * a.Lq + q2) * a.Hkv * a.G + hk * a.G + g2) * a.D + d] = (T)(v * ml[0][r][0]);
+    }
+  }
+}
+
+// ---- joins the key ranges: one wave per row (lane = channels)
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+  const int R = a.G * a.Lq;
+  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (w >= (int64_t)a.B * a.Hkv * R) return;
+  const int lane = threadIdx.x & 63;
+  const int bh = (int)(w / R), row = (int)(w - (int64_t)bh * R);
+  const int64_t p0 = (int64_t)bh * a.nsplit * R + row;
+  float mt = -INFINITY;
+  for (int s = 0; s < a.nsplit; ++s) mt = fmaxf(mt, a.part_ml[2 * (p0 + (int64_t)s * R)]);
+  const float ms = mt == -INFINITY ? 0.f : mt;
+  constexpr int PL = (DP + 63) / 64;
+  float lt = 0.f, o[PL];
+#pragma unroll
+  for (int k = 0; k < PL; ++k) o[k] = 0.f;
+  for (int s = 0; s < a.nsplit; ++s) {
+    const int64_t p = p0 + (int64_t)s * R;
+    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * p] - ms);
+    lt += a.part_ml[2 * p + 1] * f;
+#pragma unroll
+    for (int k = 0; k < PL; ++k)
+      if (lane + 64 * k < DP) o[k] += a.part[p * DP + lane + 64 * k] * f;
+  }
+  const bool some = lt > 0.f || lt != lt;
+  const float inv = some ? 1.f / lt : 0.f;
+  const int b = bh / a.Hkv, hk = bh - b * a.Hkv, qi = row / a.G, g = row - qi * a.G;
+  T* out = reinterpret_cast<T*>(a.o) + (((int64_t)b * a.Lq + qi) * a.Hkv * a.G + hk * a.G + g) * a.D;
+#pragma unroll
+  for (int k = 0; k < PL; ++k)
+    if (lane + 64 * k < a.D) out[lane + 64 * k] = (T)(o[k] * inv);
+  if (a.lse && lane == 0) a.lse[(int64_t)bh * R + row] = some ? mt + log2f(lt) : INFINITY;
+}
+
+template <typename T, int DP, int MASK>
+void fwd_launch(const AttnArgs& a, hipStream_t s) {
+  const int64_t R = (int64_t)a.G * a.Lq;
+  const int64_t n = (R <= 32 ? 1 : (R + 127) / 128) * a.nsplit * a.B * a.Hkv;
+  const unsigned grid = raft_cdiv(n, 8) * 8;
+  if (R <= 32) attn_few_kernel<T, DP, MASK><<<grid, 256, 0, s>>>(a);
+  else attn_fwd_kernel<T, DP, MASK><<<grid, 256, 0, s>>>(a);
+  if (a.nsplit > 1) attn_join_kernel<T, DP><<<raft_cdiv((int64_t)a.B * a.Hkv * R, 4), 256, 0, s>>>(a);
+}
+template <typename T, int DP>
+void fwd_mask(const AttnArgs& a, hipStream_t s) {
+  if (a.mask_mode == 0) fwd_launch<T, DP, 0>(a, s);
+  else if (a.mask_mode == 1) fwd_launch<T, DP, 1>(a, s);
+  else fwd_launch<T, DP, 2>(a, s);
+}
+template <typename T>
+void fwd_dim(const AttnArgs& a, hipStream_t s) {
+  if (a.DP == 32) fwd_mask<T, 32>(a, s);
+  else if (a.DP == 64) fwd_mask<T, 64>(a, s);
+  else if (a.DP == 96) fwd_mask<T, 96>(a, s);
+  else fwd_mask<T, 128>(a, s);
+}
+
+}  // namespace attn_detail
+
+int attn_splits(const AttnArgs& a) {
+  // Enough workgroups for the 256 CUs: key ranges are split (and joined by a second launch) when the
+  // row tiles alone leave CUs idle; a range keeps at least 256 keys so the join stays small.
+  const int64_t R = (int64_t)a.G * a.Lq;
+  const int64_t n = (R <= 32 ? 1 : (R + 127) / 128) * a.B * a.Hkv;
+  const int64_t want = R <= 32 ? 512 : 256;
+  int64_t s = n > 0 ? want / n : 1;
+  s = std::min<int64_t>(s, (a.Lk + 255) / 256);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(s, 64));
+}
+
+void launch_attn_fwd(const AttnArgs& a, hipStream_t s) {
+  if (a.dtype == 0) attn_detail::fwd_dim<__bf16>(a, s);
+  else if (a.dtype == 1) attn_detail::fwd_dim<_Float16>(a, s);
+  else attn_detail::fwd_dim<float>(a, s);
+}

@@ -453,3 +453,32 @@ bool launch_gather_cast(const GatherSrcs& s, const int32_t* idx, void* out, int6
 // ot: 0 bf16, 1 fp16, 2 fp32
 bool launch_image_prep(const float* a, const float* b, void* out, int B, int64_t HW, int ot,
                        hipStream_t stream);
+
+// ---- softmax attention over tokens (attn_fwd.hip, attn_bwd.hip).  Strides in elements; the last
+// dimension is contiguous, every row starts on 16 bytes.  o (B, Lq, Hkv * G, D) contiguous; lse, delta
+// (B, Hkv, G * Lq) in log2 units / fp32, rows position-major over the G heads of a key head.
+struct AttnArgs {
+  const void *q, *k, *v;
+  void* o;
+  float* lse;             // nullable in the forward
+  int64_t q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh;
+  int B, Lq, Lk, Hkv, G, D, DP;
+  int dtype;              // 0 bf16, 1 fp16, 2 fp32
+  float scale, scale_log2;
+  int causal;
+  const int *lengths, *q_offset;      // (B), nullable
+  const uint8_t* mask;    // nonzero = seen; mode 0 none, 1 over keys (b, key), 2 over (b, h, query, key)
+  int mask_mode;
+  int64_t m_sb, m_sh, m_sq, m_sk;
+  int nsplit;             // key ranges; > 1: partial outputs (B, Hkv, nsplit, R, DP) and (.., 2) max / sum
+  float *part, *part_ml;
+  // backward
+  const void* dout;       // (B, Lq, H, D), strides d_*
+  int64_t d_sb, d_sl, d_sh;
+  float* delta;
+  uint32_t* amax;         // fp16 only: largest |dout row| and |v row| (2-norms, as float bits)
+  void *dq, *dk, *dv;     // contiguous (B, L, heads, D)
+};
+int attn_splits(const AttnArgs& a);
+void launch_attn_fwd(const AttnArgs& a, hipStream_t s);
+void launch_attn_bwd(const AttnArgs& a, hipStream_t s);

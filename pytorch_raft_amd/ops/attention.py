@@ -1,0 +1,123 @@
+"""Softmax attention over tokens (flattened feature maps, or any sequence): HIP kernels + torch oracle.
+
+``attention(q, k, v)``: q (B, Lq, H, D), k and v (B, Lk, Hkv, D) -> (B, Lq, H, D), where query head h
+reads key head ``h // (H // Hkv)``.  A channels_last feature map (B, C, h, w) is such a tensor without
+a copy: ``x.permute(0, 2, 3, 1).reshape(B, h * w, heads, C // heads)``; so are the parts of one q|k|v
+projection.
+
+* ``scale``: of the scores, default ``D ** -0.5``; positive.
+* ``lengths`` (B,) int32: item b holds keys 0 .. lengths[b] - 1; what lies behind is not read.
+* ``causal``: query i of item b stands at key position ``q_offset[b] + i`` and sees the keys up to it;
+  ``q_offset`` (B,) int32 defaults to ``Lk - Lq`` (the last query sees the last key).  A step over
+  caches filled to ``lengths`` passes ``q_offset = lengths - Lq``.  Without ``causal`` it changes nothing.
+* ``mask``: bool, broadcastable to (B, H, Lq, Lk), True where a query sees a key.  Keys hidden by a
+  mask that is the same for all queries and heads (a padding mask (B, 1, 1, Lk)) may hold anything; under a mask that
+  differs between queries, and under ``causal``, keys and values must be finite.
+
+A query that sees no key gets zeros, and zero gradients.  bf16, fp16 and fp32; sums, maxima and
+accumulators are fp32, the probabilities are rounded to the inputs' type for their product with v.
+Differentiable in q, k and v (the backward recomputes the probabilities from a saved log-sum-exp; the
+same inputs give the same bits).  Head sizes up to 128 (others than multiples of 8 are padded by a
+copy).  Calls with at most 32 rows (H / Hkv * Lq), e.g. single tokens over a cache, run a kernel that
+splits the keys.
+
+The all-pairs correlation (ops/corr.py) is the same product of two feature maps without the softmax.
+"""
+import torch
+import torch.nn.functional as F
+
+from . import _ext
+
+MAX_HEAD = 128
+
+
+def torch_attention(q, k, v, scale=None, causal=False, mask=None, lengths=None, q_offset=None):
+    """Plain implementation in the inputs' precision (also the CPU path)."""
+    b, lq, h, d = q.shape
+    lk, hkv = k.shape[1:3]
+    scale = d ** -0.5 if scale is None else scale
+    dev = q.device
+    j = torch.arange(lk, device=dev)
+    see = torch.ones(b, 1, lq, lk, dtype=torch.bool, device=dev)
+    if lengths is not None:
+        see = see & (j < lengths[:, None])[:, None, None]
+    if causal:
+        first = q_offset if q_offset is not None else torch.full((b,), lk - lq, device=dev)
+        pos = first[:, None] + torch.arange(lq, device=dev)
+        see = see & (j <= pos[..., None])[:, None]
+    if mask is not None:
+        see = see & mask
+    # keys that nobody sees may hold anything
+    used = see.any(1).any(1)[:, :, None, None]
+    k = torch.where(used, k, torch.zeros_like(k)).repeat_interleave(h // hkv, 2)
+    v = torch.where(used, v, torch.zeros_like(v)).repeat_interleave(h // hkv, 2)
+    s = torch.matmul(q.transpose(1, 2).contiguous(), k.permute(0, 2, 3, 1).contiguous()) * scale
+    some = see.any(-1, keepdim=True)
+    s = s.masked_fill(~see, float('-inf')).masked_fill(~some, 0.)
+    p = torch.softmax(s, -1).masked_fill(~some, 0.) if lk else s
+    return torch.matmul(p, v.transpose(1, 2).contiguous()).transpose(1, 2)
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, scale, causal, mask, lengths, q_offset):
+        need = any(ctx.needs_input_grad[:3])
+        out, lse = _ext.ops().attn_fwd(q, k, v, scale, causal, mask, lengths, q_offset, need)
+        if need:
+            ctx.save_for_backward(q, k, v, out, lse, mask, lengths, q_offset)
+            ctx.p = (scale, causal)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse, mask, lengths, q_offset = ctx.saved_tensors
+        dq, dk, dv = _ext.ops().attn_bwd(dout, q, k, v, out, lse, *ctx.p, mask, lengths, q_offset)
+        return dq, dk, dv, None, None, None, None, None
+
+
+def _check(q, k, v, scale, mask, lengths, q_offset):
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
+        raise ValueError('q must be (B, Lq, H, D), k and v (B, Lk, Hkv, D); got %s, %s, %s'
+                         % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    b, lq, h, d = q.shape
+    if k.shape[0] != b or k.shape[3] != d:
+        raise ValueError('q %s and k %s disagree on batch or head size' % (tuple(q.shape), tuple(k.shape)))
+    if not k.shape[2] or not h or h % k.shape[2]:
+        raise ValueError('the %d query heads must be a multiple of the %d key heads' % (h, k.shape[2]))
+    if not 1 <= d <= MAX_HEAD:
+        raise ValueError('head size must be 1 .. %d, got %d' % (MAX_HEAD, d))
+    if not (q.dtype == k.dtype == v.dtype):
+        raise TypeError('q, k and v must have one dtype, got %s, %s, %s' % (q.dtype, k.dtype, v.dtype))
+    if not 0 < scale < float('inf'):
+        raise ValueError('scale must be positive and finite, got %r' % scale)
+    if mask is not None:
+        if mask.dtype != torch.bool:
+            raise TypeError('mask must be bool (True = seen), got %s' % mask.dtype)
+        if mask.dim() > 4 or any(m not in (1, n) for m, n in zip(mask.shape[::-1], (k.shape[1], lq, h, b))):
+            raise ValueError('mask %s does not broadcast to %s' % (tuple(mask.shape), (b, h, lq, k.shape[1])))
+    for name, t in (('lengths', lengths), ('q_offset', q_offset)):
+        if t is not None and (t.dtype != torch.int32 or t.shape != (b,)):
+            raise ValueError('%s must be int32 of shape (%d,), got %s %s' % (name, b, t.dtype, tuple(t.shape)))
+    for name, t in (('k', k), ('v', v), ('mask', mask), ('lengths', lengths), ('q_offset', q_offset)):
+        if t is not None and t.device != q.device:
+            raise ValueError('%s is on %s, q on %s' % (name, t.device, q.device))
+
+
+def attention(q, k, v, scale=None, causal=False, mask=None, lengths=None, q_offset=None, impl='auto'):
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    _check(q, k, v, scale, mask, lengths, q_offset)
+    if impl != 'torch' and _ext.device_ok(q) and _ext.gpu_path_enabled(required=(impl == 'hip')):
+        if q.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+            raise TypeError('attention runs in bf16, fp16 and fp32, got %s' % q.dtype)
+        d = q.shape[-1]
+        pad = -d % 8
+        if pad:
+            q, k, v = (F.pad(t, (0, pad)) for t in (q, k, v))
+        if mask is not None:
+            mask = mask.expand(q.shape[0], q.shape[2], q.shape[1], k.shape[1])
+        out = _Attention.apply(q, k, v, scale, bool(causal), mask,
+                               None if lengths is None else lengths.contiguous(),
+                               None if q_offset is None else q_offset.contiguous())
+        return out[..., :d] if pad else out
+    return torch_attention(q, k, v, scale, causal, mask, lengths, q_offset)
