@@ -167,14 +167,142 @@ std::vector<Tensor> attn_bwd(const Tensor& dout0, const Tensor& q0, const Tensor
   return {dq, dk, dv};
 }
 
+// ------------------------------------------------------------------ root-mean-square norm
+RmsArgs rms_args(const Tensor& x, const Tensor& w, double eps) {
+  TORCH_CHECK(x.is_cuda() && w.device() == x.device(), "x and weight must be on one GPU");
+  TORCH_CHECK(x.dim() == 2 && x.is_contiguous(), "x must be contiguous (rows, C)");
+  TORCH_CHECK(x.size(1) >= 1 && x.size(1) <= 16384, "rms norm takes 1 to 16384 channels, got ", x.size(1));
+  TORCH_CHECK(w.dim() == 1 && w.size(0) == x.size(1) && w.is_contiguous() &&
+                  (w.scalar_type() == at::kFloat || w.scalar_type() == x.scalar_type()),
+              "weight must be contiguous (C,), float32 or the dtype of x");
+  TORCH_CHECK(std::isfinite(eps) && eps >= 0, "eps must be finite and not negative");
+  RmsArgs a = {};
+  a.dtype = dtype_code(x, "x");
+  a.rows = x.size(0);
+  a.C = (int)x.size(1);
+  a.eps = (float)eps;
+  a.w = w.data_ptr();
+  a.w_f32 = w.scalar_type() == at::kFloat;
+  a.x = x.data_ptr();
+  return a;
+}
+void check_like(const Tensor& t, const Tensor& x, const char* name) {
+  TORCH_CHECK(t.device() == x.device() && t.scalar_type() == x.scalar_type() && t.sizes() == x.sizes() && t.is_contiguous(),
+              name, " must match x (device, dtype, shape, contiguous)");
+}
+
+// -> {y, h (the sum; empty without a residual), 1 / rms (rows) or empty}
+std::vector<Tensor> rms_fwd(const Tensor& x, const Tensor& w, OptTensor residual, double eps, bool need_rstd) {
+  RmsArgs a = rms_args(x, w, eps);
+  c10::DeviceGuard g(x.device());
+  const auto f32 = x.options().dtype(at::kFloat);
+  Tensor y = at::empty_like(x), h = given(residual) ? at::empty_like(x) : at::empty({0}, x.options());
+  Tensor rstd = at::empty({need_rstd ? x.size(0) : 0}, f32);
+  if (given(residual)) {
+    check_like(*residual, x, "residual");
+    a.r = residual->data_ptr();
+    a.h = h.data_ptr();
+  }
+  a.y = y.data_ptr();
+  a.rstd = need_rstd ? rstd.data_ptr<float>() : nullptr;
+  if (a.rows > 0) launch_rms_fwd(a, cur_stream());
+  return {y, h, rstd};
+}
+
+// -> {q int8, scale fp32 (rows), h or empty}
+std::vector<Tensor> rms_fwd_int8(const Tensor& x, const Tensor& w, OptTensor residual, double eps) {
+  RmsArgs a = rms_args(x, w, eps);
+  c10::DeviceGuard g(x.device());
+  Tensor q = at::empty(x.sizes(), x.options().dtype(at::kChar)), h = given(residual) ? at::empty_like(x) : at::empty({0}, x.options());
+  Tensor scale = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
+  if (given(residual)) {
+    check_like(*residual, x, "residual");
+    a.r = residual->data_ptr();
+    a.h = h.data_ptr();
+  }
+  a.y = q.data_ptr();
+  a.rstd = scale.data_ptr<float>();
+  if (a.rows > 0) launch_rms_int8(a, cur_stream());
+  return {q, scale, h};
+}
+
+// h: the forward's sum (or x) -> {dx (also the residual's gradient), dw}
+std::vector<Tensor> rms_bwd(const Tensor& dy, OptTensor dh, const Tensor& h, const Tensor& w, const Tensor& rstd) {
+  RmsArgs a = rms_args(h, w, 0.0);
+  c10::DeviceGuard g(h.device());
+  check_like(dy, h, "dy");
+  TORCH_CHECK(rstd.device() == h.device() && rstd.scalar_type() == at::kFloat && rstd.is_contiguous() && rstd.dim() == 1 && rstd.size(0) == h.size(0),
+              "rstd must be the forward's");
+  if (given(dh)) check_like(*dh, h, "dh");
+  Tensor dx = at::empty_like(h), dw = at::empty_like(w);
+  if (a.rows == 0) return {dx, dw.zero_()};
+  a.parts = rms_parts(a.rows, a.C);
+  Tensor part = at::empty({a.parts, (int64_t)a.C}, h.options().dtype(at::kFloat));
+  a.h = h.data_ptr();
+  a.dy = dy.data_ptr();
+  a.dh = given(dh) ? dh->data_ptr() : nullptr;
+  a.rstd = rstd.data_ptr<float>();
+  a.dx = dx.data_ptr();
+  a.dw = dw.data_ptr();
+  a.part = part.data_ptr<float>();
+  launch_rms_bwd(a, cur_stream());
+  return {dx, dw};
+}
+
+// ------------------------------------------------------------------ 8-bit integer product
+void check_vec(const Tensor& t, const Tensor& x, int64_t n, const char* name) {
+  TORCH_CHECK(t.device() == x.device() && t.scalar_type() == at::kFloat && t.dim() == 1 && t.size(0) == n && t.is_contiguous(),
+              name, " must be contiguous float32 of shape (", n, ",) on the device of x");
+}
+
+// out_dtype: 0 bf16, 1 fp16, 2 fp32
+Tensor int8_mm(const Tensor& x, const Tensor& xs, const Tensor& w, const Tensor& ws, OptTensor bias, int64_t out_dtype) {
+  TORCH_CHECK(x.is_cuda() && w.device() == x.device(), "x and w must be on one GPU");
+  TORCH_CHECK(x.scalar_type() == at::kChar && w.scalar_type() == at::kChar, "x and w must be int8");
+  TORCH_CHECK(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1) && x.is_contiguous() && w.is_contiguous(),
+              "x must be contiguous (M, K), w contiguous (N, K)");
+  TORCH_CHECK(out_dtype >= 0 && out_dtype <= 2, "out_dtype: 0 bf16, 1 fp16, 2 fp32");
+  const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
+  TORCH_CHECK(K <= 131071, "int8_mm: K past 131071 could overflow the 32-bit sums");
+  TORCH_CHECK(M < (int64_t(1) << 28) && N < (int64_t(1) << 28) && ((M + 63) / 64) * ((N + 63) / 64) < (int64_t(1) << 23),
+              "int8_mm: too many outputs for one call");
+  check_vec(xs, x, M, "xs");
+  check_vec(ws, x, N, "ws");
+  if (given(bias)) check_vec(*bias, x, N, "bias");
+  c10::DeviceGuard g(x.device());
+  Tensor out = at::empty({M, N}, x.options().dtype(out_dtype == 0 ? at::kBFloat16 : out_dtype == 1 ? at::kHalf : at::kFloat));
+  if (M == 0 || N == 0) return out;
+  Int8Args a = {};
+  a.x = x.data_ptr<int8_t>();
+  a.w = w.data_ptr<int8_t>();
+  a.xs = xs.data_ptr<float>();
+  a.ws = ws.data_ptr<float>();
+  a.bias = given(bias) ? bias->data_ptr<float>() : nullptr;
+  a.out = out.data_ptr();
+  a.M = (int)M;
+  a.N = (int)N;
+  a.K = (int)K;
+  a.dtype = (int)out_dtype;
+  launch_int8_mm(a, cur_stream());
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(raft_amd, m) {
   m.def("attn_fwd(Tensor q, Tensor k, Tensor v, float scale, bool causal, Tensor? mask, Tensor? lengths, Tensor? q_offset, bool need_lse) -> Tensor[]");
   m.def("attn_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, float scale, bool causal, Tensor? mask, Tensor? lengths, Tensor? q_offset) -> Tensor[]");
+  m.def("rms_fwd(Tensor x, Tensor w, Tensor? residual, float eps, bool need_rstd) -> Tensor[]");
+  m.def("rms_fwd_int8(Tensor x, Tensor w, Tensor? residual, float eps) -> Tensor[]");
+  m.def("rms_bwd(Tensor dy, Tensor? dh, Tensor h, Tensor w, Tensor rstd) -> Tensor[]");
+  m.def("int8_mm(Tensor x, Tensor xs, Tensor w, Tensor ws, Tensor? bias, int out_dtype) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(raft_amd, CUDA, m) {
   m.impl("attn_fwd", &attn_fwd);
   m.impl("attn_bwd", &attn_bwd);
+  m.impl("rms_fwd", &rms_fwd);
+  m.impl("rms_fwd_int8", &rms_fwd_int8);
+  m.impl("rms_bwd", &rms_bwd);
+  m.impl("int8_mm", &int8_mm);
 }

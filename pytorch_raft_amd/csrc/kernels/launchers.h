@@ -482,3 +482,32 @@ struct AttnArgs {
 int attn_splits(const AttnArgs& a);
 void launch_attn_fwd(const AttnArgs& a, hipStream_t s);
 void launch_attn_bwd(const AttnArgs& a, hipStream_t s);
+
+// ---- root-mean-square norm (rms_norm.hip): rows x C, contiguous; C <= 16384
+struct RmsArgs {
+  const void *x, *r;      // r nullable
+  const void* w;          // fp32 (w_f32) or the type of x
+  int w_f32, dtype, C;
+  int64_t rows;
+  float eps;
+  void *h, *y;            // h written only with r; y: type of x, or int8
+  float* rstd;            // forward: nullable output; 8-bit form: the rows' scales
+  // backward (h, rstd: the forward's)
+  const void *dy, *dh;    // dh nullable
+  void *dx, *dw;
+  float* part;            // (parts, C)
+  int parts;
+};
+int rms_parts(int64_t rows, int C);
+void launch_rms_fwd(const RmsArgs& a, hipStream_t s);
+void launch_rms_int8(const RmsArgs& a, hipStream_t s);
+void launch_rms_bwd(const RmsArgs& a, hipStream_t s);
+
+// ---- 8-bit integer product (int8_mm.hip): x (M, K), w (N, K), out (M, N), contiguous
+struct Int8Args {
+  const int8_t *x, *w;
+  const float *xs, *ws, *bias;  // bias nullable
+  void* out;
+  int M, N, K, dtype;
+};
+void launch_int8_mm(const Int8Args& a, hipStream_t s);

@@ -1,0 +1,59 @@
+"""8-bit integer linear layer (a 1x1 conv over NHWC pixels) with a scale for each token and each output
+channel: HIP kernel + torch oracle.
+
+``int8_linear(x, x_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16)``:
+    out[..., n] = x_scale[...] * w_scale[n] * sum_k x[..., k] * w[n, k]  (+ bias[n])
+x (..., K) int8 and x_scale (...) fp32 come from ``rms_norm_int8`` (ops/rms_norm.py); w (N, K) int8 and
+w_scale (N,) fp32 from ``quantize_weight`` once; bias (N,) fp32.  The sum is exact (int32; K up to
+131071), scaled in fp32 and rounded once to ``out_dtype`` (bf16, fp16 or fp32).  For inference: no
+gradient.  Operands whose rows start on 16 bytes (K a multiple of 16) take the fastest loads.
+"""
+import torch
+
+from . import _ext
+
+MAX_K = 131071
+_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def quantize_weight(weight):
+    """(N, K) floating weight -> (int8 (N, K), fp32 scale (N,)), symmetric per output channel; once, not per call."""
+    if weight.dim() != 2 or not weight.is_floating_point():
+        raise ValueError('weight must be a floating (N, K) tensor, got %s %s' % (weight.dtype, tuple(weight.shape)))
+    w = weight.detach().float()
+    top = w.abs().amax(1, keepdim=True) if w.shape[1] else w.new_zeros(w.shape[0], 1)
+    q = torch.round(w * torch.where(top == 0, torch.zeros_like(top), 127 / top)).clamp_(-127, 127)
+    return q.to(torch.int8), (top / 127).squeeze(1)
+
+
+def torch_int8_linear(x, x_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16):
+    """Plain implementation (also the CPU path); 64-bit sums are exact like the kernel's."""
+    y = (torch.matmul(x.double(), w.double().t()).float() * x_scale[..., None]) * w_scale
+    return (y if bias is None else y + bias).to(out_dtype)
+
+
+def int8_linear(x, x_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16, impl='auto'):
+    if x.dtype != torch.int8 or w.dtype != torch.int8:
+        raise TypeError('x and w must be int8, got %s and %s' % (x.dtype, w.dtype))
+    if out_dtype not in _CODES:
+        raise TypeError('out_dtype must be bfloat16, float16 or float32, got %s' % out_dtype)
+    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
+        raise ValueError('x must be (..., K), w (N, K); got %s, %s' % (tuple(x.shape), tuple(w.shape)))
+    n, k = w.shape
+    if k > MAX_K:
+        raise ValueError('K = %d could overflow the 32-bit sums (at most %d)' % (k, MAX_K))
+    for name, t, shape in (('x_scale', x_scale, x.shape[:-1]), ('w_scale', w_scale, (n,)), ('bias', bias, (n,))):
+        if t is None and name == 'bias':
+            continue
+        if t.dtype != torch.float32 or t.shape != tuple(shape):
+            raise ValueError('%s must be float32 of shape %s, got %s %s' % (name, tuple(shape), t.dtype, tuple(t.shape)))
+        if torch.is_grad_enabled() and t.requires_grad:
+            raise RuntimeError('int8_linear has no gradient (%s requires one): call it under torch.no_grad()' % name)
+    for name, t in (('x_scale', x_scale), ('w', w), ('w_scale', w_scale), ('bias', bias)):
+        if t is not None and t.device != x.device:
+            raise ValueError('%s is on %s, x on %s' % (name, t.device, x.device))
+    if impl != 'torch' and _ext.device_ok(x) and _ext.gpu_path_enabled(required=(impl == 'hip')):
+        out = _ext.ops().int8_mm(x.reshape(x.shape[:-1].numel(), k).contiguous(), x_scale.reshape(-1).contiguous(), w.contiguous(),
+                                 w_scale.contiguous(), None if bias is None else bias.contiguous(), _CODES[out_dtype])
+        return out.view(*x.shape[:-1], n)
+    return torch_int8_linear(x, x_scale, w, w_scale, bias, out_dtype)

@@ -1,0 +1,109 @@
+"""Root-mean-square norm over the channels, with the residual's addition: HIP kernels + torch oracle.
+
+``rms_norm(x, weight)`` -> y = x / sqrt(mean x^2 + eps) * weight.
+``rms_norm(x, weight, residual=r)`` -> (y, h): h = x + r, rounded to the type of x (it is the stream
+that the next residual adds to), and y is the norm of h as rounded.  Differentiable in x, residual and
+weight (the encoders' fused norms, ops/encoder.py, are the per-image and per-batch counterparts).
+
+``rms_norm_int8(x, weight, residual=None)`` -> (q, scale, h): the same norm with an 8-bit output for
+``int8_linear`` (ops/int8.py): q = rint(y * 127 / max|y|) int8 with one fp32 scale = max|y| / 127 per
+row (both from the unrounded fp32 y; an all-zero row has scale 0; a row with a NaN has scale NaN).
+h is None without a residual.  For inference: it has no gradient.
+
+x (..., C) bf16, fp16 or fp32, C up to 16384; weight (C,) fp32 or the type of x; statistics in fp32.
+"""
+import torch
+
+from . import _ext
+
+MAX_CHANNELS = 16384
+
+
+def _torch_norm(x, weight, residual, eps):
+    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+    h = x if residual is None else (x.to(wide) + residual.to(wide)).to(x.dtype)
+    f = h.to(wide)
+    return f * torch.rsqrt(f.square().mean(-1, keepdim=True) + eps) * weight.to(wide), h
+
+
+def torch_rms_norm(x, weight, residual=None, eps=1e-6):
+    """Plain implementation (also the CPU path)."""
+    y, h = _torch_norm(x, weight, residual, eps)
+    y = y.to(x.dtype)
+    return y if residual is None else (y, h)
+
+
+def torch_rms_norm_int8(x, weight, residual=None, eps=1e-6):
+    y, h = _torch_norm(x, weight, residual, eps)
+    top = y.abs().amax(-1, keepdim=True)
+    q = torch.round(y * torch.where(top == 0, torch.zeros_like(top), 127 / top)).clamp(-127, 127)
+    return q.nan_to_num(0.).to(torch.int8), (top / 127).squeeze(-1), None if residual is None else h
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        need = any(ctx.needs_input_grad[:3])
+        y, h, rstd = _ext.ops().rms_fwd(x, weight, residual, eps, need)
+        ctx.set_materialize_grads(False)
+        ctx.residual = residual is not None
+        if need:
+            ctx.save_for_backward(h if ctx.residual else x, weight, rstd)
+        return (y, h) if ctx.residual else y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh=None):
+        h, weight, rstd = ctx.saved_tensors
+        dh = None if dh is None else dh.contiguous()
+        if dy is None:
+            return dh, None, dh, None
+        dx, dw = _ext.ops().rms_bwd(dy.contiguous(), dh, h, weight, rstd)
+        return dx, dw, dx if ctx.residual else None, None
+
+
+def _check(x, weight, residual, eps):
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_CHANNELS:
+        raise ValueError('x must be (..., C) with 1 .. %d channels, got %s' % (MAX_CHANNELS, tuple(x.shape)))
+    if weight.shape != x.shape[-1:]:
+        raise ValueError('weight %s does not match the channels of x %s' % (tuple(weight.shape), tuple(x.shape)))
+    if weight.dtype not in (torch.float32, x.dtype):
+        raise TypeError('weight must be float32 or %s, got %s' % (x.dtype, weight.dtype))
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError('residual %s %s does not match x %s %s'
+                         % (residual.dtype, tuple(residual.shape), x.dtype, tuple(x.shape)))
+    if not 0 <= eps < float('inf'):
+        raise ValueError('eps must be finite and not negative, got %r' % eps)
+    for name, t in (('weight', weight), ('residual', residual)):
+        if t is not None and t.device != x.device:
+            raise ValueError('%s is on %s, x on %s' % (name, t.device, x.device))
+
+
+def _on_gpu(x, impl):
+    if impl == 'torch' or not _ext.device_ok(x) or not _ext.gpu_path_enabled(required=(impl == 'hip')):
+        return False
+    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError('rms_norm runs in bf16, fp16 and fp32, got %s' % x.dtype)
+    return True
+
+
+def rms_norm(x, weight, residual=None, eps=1e-6, impl='auto'):
+    _check(x, weight, residual, eps)
+    if not _on_gpu(x, impl):
+        return torch_rms_norm(x, weight, residual, eps)
+    c = x.shape[-1]
+    out = _RmsNorm.apply(x.reshape(-1, c).contiguous(), weight.contiguous(),
+                         None if residual is None else residual.reshape(-1, c).contiguous(), float(eps))
+    return out.view(x.shape) if residual is None else tuple(t.view(x.shape) for t in out)
+
+
+def rms_norm_int8(x, weight, residual=None, eps=1e-6, impl='auto'):
+    _check(x, weight, residual, eps)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+        raise RuntimeError('rms_norm_int8 has no gradient: call it under torch.no_grad()')
+    if not _on_gpu(x, impl):
+        return torch_rms_norm_int8(x, weight, residual, eps)
+    c = x.shape[-1]
+    q, scale, h = _ext.ops().rms_fwd_int8(x.reshape(-1, c).contiguous(), weight.contiguous(),
+                                          None if residual is None else residual.reshape(-1, c).contiguous(), float(eps))
+    return q.view(x.shape), scale.view(x.shape[:-1]), None if residual is None else h.view(x.shape)
