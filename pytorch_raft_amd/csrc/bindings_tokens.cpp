@@ -2,6 +2,7 @@
 // (forward, backward, 8-bit output), 8-bit integer product.  Same rules as bindings.cpp: every
 // argument is checked on the host before a launch, kernels run on the current stream of the tensors'
 // device, outputs and workspaces come from torch's allocator.
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
@@ -153,13 +154,19 @@ std::vector<Tensor> attn_bwd(const Tensor& dout0, const Tensor& q0, const Tensor
   Tensor dk = at::empty(k.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
   Tensor dv = at::empty(k.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
   if (a.B == 0 || a.Lq == 0 || a.Lk == 0) return {dq.zero_(), dk.zero_(), dv.zero_()};
-  Tensor ws = at::empty({(int64_t)a.B * a.Hkv * R + 2}, q.options().dtype(at::kFloat));
+  attn_bwd_plan(a);
+  // one workspace: split parts (first: they want 16 bytes), delta, norms
+  const int64_t n_kv = a.nsplit_kv > 1 ? 2 * a.nsplit_kv * dk.numel() : 0, n_q = a.nsplit_q > 1 ? a.nsplit_q * dq.numel() : 0;
+  const int64_t n_rows = (int64_t)a.B * a.Hkv * R;
+  Tensor ws = at::empty({n_kv + n_q + n_rows + (a.dtype == 1 ? 2 * a.nprep : 0)}, q.options().dtype(at::kFloat));
+  a.part = ws.data_ptr<float>();
+  a.part_q = a.part + n_kv;
   a.o = out.data_ptr();
   a.lse = lse.data_ptr<float>();
   a.dout = dout.data_ptr();
   a.d_sb = stride_of(dout, 0), a.d_sl = stride_of(dout, 1), a.d_sh = stride_of(dout, 2);
-  a.delta = ws.data_ptr<float>();
-  a.amax = reinterpret_cast<uint32_t*>(a.delta + (int64_t)a.B * a.Hkv * R);
+  a.delta = a.part_q + n_q;
+  a.amax = reinterpret_cast<uint32_t*>(a.delta + n_rows);
   a.dq = dq.data_ptr();
   a.dk = dk.data_ptr();
   a.dv = dv.data_ptr();
@@ -287,9 +294,207 @@ Tensor int8_mm(const Tensor& x, const Tensor& xs, const Tensor& w, const Tensor&
   return out;
 }
 
+// ------------------------------------------------------------------ the public operators
+// Autograd nodes in C++: for the short launches of small batches the Python form of a node costs more
+// host time than the kernels run (a norm's forward and backward: 140 us issued from Python nodes).
+using torch::autograd::AutogradContext;
+using torch::autograd::Variable;
+using torch::autograd::variable_list;
+
+bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+void once_only(const char* name) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), name, " has no second derivative (create_graph)");
+}
+
+struct AttentionNode : public torch::autograd::Function<AttentionNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, double scale, bool causal,
+                        OptTensor mask, OptTensor lengths, OptTensor q_offset) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto r = attn_fwd(q, k, v, scale, causal, mask, lengths, q_offset, true);
+    const auto opt = [](OptTensor t) { return given(t) ? *t : Tensor(); };
+    ctx->save_for_backward({q, k, v, r[0], r[1], opt(mask), opt(lengths), opt(q_offset)});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["causal"] = causal;
+    return r[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once_only("attention");
+    const auto s = ctx->get_saved_variables();
+    const auto opt = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+    auto r = attn_bwd(grads[0], s[0], s[1], s[2], s[3], s[4], ctx->saved_data["scale"].toDouble(), ctx->saved_data["causal"].toBool(),
+                      opt(s[5]), opt(s[6]), opt(s[7]));
+    return {r[0], r[1], r[2], Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// q (B, Lq, H, D), k, v (B, Lk, Hkv, D), mask broadcastable to (B, H, Lq, Lk); scale 0: D ** -0.5
+Tensor attention(const Tensor& q0, const Tensor& k0, const Tensor& v0, std::optional<double> scale0, bool causal, OptTensor mask0,
+                 OptTensor lengths, OptTensor q_offset) {
+  TORCH_CHECK_VALUE(q0.dim() == 4 && k0.dim() == 4 && v0.sizes() == k0.sizes(), "q must be (B, Lq, H, D), k and v (B, Lk, Hkv, D); got ",
+                    q0.sizes(), ", ", k0.sizes(), ", ", v0.sizes());
+  TORCH_CHECK_TYPE(q0.scalar_type() == k0.scalar_type() && q0.scalar_type() == v0.scalar_type(),
+                   "q, k and v must have one dtype, got ", q0.scalar_type(), ", ", k0.scalar_type(), ", ", v0.scalar_type());
+  TORCH_CHECK_TYPE(q0.scalar_type() == at::kBFloat16 || q0.scalar_type() == at::kHalf || q0.scalar_type() == at::kFloat,
+                   "attention runs in bf16, fp16 and fp32, got ", q0.scalar_type());
+  const int64_t B = q0.size(0), Lq = q0.size(1), H = q0.size(2), D = q0.size(3), Lk = k0.size(1), Hkv = k0.size(2);
+  TORCH_CHECK_VALUE(k0.size(0) == B && k0.size(3) == D, "q ", q0.sizes(), " and k ", k0.sizes(), " disagree on batch or head size");
+  TORCH_CHECK_VALUE(Hkv > 0 && H > 0 && H % Hkv == 0, "the ", H, " query heads must be a multiple of the ", Hkv, " key heads");
+  TORCH_CHECK_VALUE(D >= 1 && D <= 128, "head size must be 1 .. 128, got ", D);
+  const double scale = scale0.has_value() ? *scale0 : 1.0 / std::sqrt((double)D);
+  TORCH_CHECK_VALUE(std::isfinite(scale) && scale > 0, "scale must be positive and finite, got ", scale);
+  const auto on = [&](const Tensor& t, const char* name) {
+    TORCH_CHECK_VALUE(t.device() == q0.device(), name, " is on ", t.device(), ", q on ", q0.device());
+  };
+  on(k0, "k"), on(v0, "v");
+  const auto ints = [&](OptTensor t, const char* name) -> std::optional<Tensor> {
+    if (!given(t)) return std::nullopt;
+    on(*t, name);
+    TORCH_CHECK_VALUE(t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == B, name, " must be int32 of shape (", B, ",), got ",
+                      t->scalar_type(), " ", t->sizes());
+    return t->contiguous();
+  };
+  const auto ln = ints(lengths, "lengths"), qo = ints(q_offset, "q_offset");
+  std::optional<Tensor> mask;
+  if (given(mask0)) {
+    on(*mask0, "mask");
+    TORCH_CHECK_TYPE(mask0->scalar_type() == at::kBool, "mask must be bool (True = seen), got ", mask0->scalar_type());
+    const int64_t want[4] = {B, H, Lq, Lk}, nd = mask0->dim();
+    bool fits = nd <= 4;
+    for (int64_t d = 0; fits && d < nd; ++d) fits = mask0->size(nd - 1 - d) == 1 || mask0->size(nd - 1 - d) == want[3 - d];
+    TORCH_CHECK_VALUE(fits, "mask ", mask0->sizes(), " does not broadcast to (", B, ", ", H, ", ", Lq, ", ", Lk, ")");
+    mask = mask0->expand({B, H, Lq, Lk});
+  }
+  Tensor q = q0, k = k0, v = v0;
+  const int64_t pad = (8 - D % 8) % 8;
+  if (pad) q = at::constant_pad_nd(q, {0, pad}), k = at::constant_pad_nd(k, {0, pad}), v = at::constant_pad_nd(v, {0, pad});
+  Tensor out;
+  if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(v))) {
+    out = AttentionNode::apply(q, k, v, scale, causal, mask, ln, qo);
+  } else {
+    at::AutoDispatchBelowADInplaceOrView below;
+    out = attn_fwd(q, k, v, scale, causal, mask, ln, qo, false)[0];
+  }
+  return pad ? out.narrow(3, 0, D) : out;
+}
+
+void rms_check(const Tensor& x, const Tensor& w, OptTensor residual, double eps) {
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 16384, "x must be (..., C) with 1 .. 16384 channels, got ", x.sizes());
+  TORCH_CHECK_TYPE(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf || x.scalar_type() == at::kFloat,
+                   "rms_norm runs in bf16, fp16 and fp32, got ", x.scalar_type());
+  TORCH_CHECK_VALUE(w.dim() == 1 && w.size(0) == x.size(-1), "weight ", w.sizes(), " does not match the channels of x ", x.sizes());
+  TORCH_CHECK_TYPE(w.scalar_type() == at::kFloat || w.scalar_type() == x.scalar_type(), "weight must be float32 or ", x.scalar_type(),
+                   ", got ", w.scalar_type());
+  TORCH_CHECK_VALUE(w.device() == x.device(), "weight is on ", w.device(), ", x on ", x.device());
+  if (given(residual)) {
+    TORCH_CHECK_VALUE(residual->sizes() == x.sizes() && residual->scalar_type() == x.scalar_type(), "residual ", residual->scalar_type(),
+                      " ", residual->sizes(), " does not match x ", x.scalar_type(), " ", x.sizes());
+    TORCH_CHECK_VALUE(residual->device() == x.device(), "residual is on ", residual->device(), ", x on ", x.device());
+  }
+  TORCH_CHECK_VALUE(std::isfinite(eps) && eps >= 0, "eps must be finite and not negative, got ", eps);
+}
+
+Tensor rows_of(const Tensor& t) { return t.contiguous().view({t.numel() / t.size(-1), t.size(-1)}); }
+
+// {y, h or undefined, rstd}, shaped like x
+std::vector<Tensor> rms_rows(const Tensor& x, const Tensor& w, OptTensor residual, double eps, bool need) {
+  auto r = rms_fwd(rows_of(x), w.contiguous(), given(residual) ? std::optional<Tensor>(rows_of(*residual)) : std::nullopt, eps, need);
+  r[0] = r[0].view(x.sizes());
+  if (given(residual)) r[1] = r[1].view(x.sizes());
+  return r;
+}
+
+struct RmsNormNode : public torch::autograd::Function<RmsNormNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, OptTensor residual, double eps) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto r = rms_rows(x, w, residual, eps, true);
+    ctx->set_materialize_grads(false);
+    const bool sum = given(residual);
+    ctx->saved_data["sum"] = sum;
+    ctx->save_for_backward({sum ? r[1] : x, w, r[2]});
+    if (sum) return {r[0], r[1]};
+    return {r[0]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once_only("rms_norm");
+    const auto s = ctx->get_saved_variables();
+    const bool sum = ctx->saved_data["sum"].toBool();
+    const Tensor dh = sum ? grads[1] : Tensor();
+    if (!grads[0].defined()) return {dh, Tensor(), dh, Tensor()};
+    auto r = rms_bwd(rows_of(grads[0]), dh.defined() ? std::optional<Tensor>(rows_of(dh)) : std::nullopt, rows_of(s[0]), s[1].contiguous(), s[2]);
+    const Tensor dx = r[0].view(s[0].sizes());
+    return {dx, r[1], sum ? dx : Tensor(), Tensor()};
+  }
+};
+
+Tensor rms_norm(const Tensor& x, const Tensor& w, double eps) {
+  rms_check(x, w, std::nullopt, eps);
+  if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w))) return RmsNormNode::apply(x, w, std::optional<Tensor>(), eps)[0];
+  at::AutoDispatchBelowADInplaceOrView below;
+  return rms_rows(x, w, std::nullopt, eps, false)[0];
+}
+
+std::tuple<Tensor, Tensor> rms_norm_residual(const Tensor& x, const Tensor& w, const Tensor& residual, double eps) {
+  rms_check(x, w, residual, eps);
+  if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(residual))) {
+    auto r = RmsNormNode::apply(x, w, std::optional<Tensor>(residual), eps);
+    return {r[0], r[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  auto r = rms_rows(x, w, residual, eps, false);
+  return {r[0], r[1]};
+}
+
+// {q, scale} or {q, scale, h}
+std::vector<Tensor> rms_norm_int8(const Tensor& x, const Tensor& w, OptTensor residual, double eps) {
+  rms_check(x, w, residual, eps);
+  TORCH_CHECK(!at::GradMode::is_enabled() || !(wants_grad(x) || wants_grad(w) || (given(residual) && wants_grad(*residual))),
+              "rms_norm_int8 has no gradient: call it under torch.no_grad()");
+  at::AutoDispatchBelowADInplaceOrView below;
+  auto r = rms_fwd_int8(rows_of(x), w.contiguous(), given(residual) ? std::optional<Tensor>(rows_of(*residual)) : std::nullopt, eps);
+  r[0] = r[0].view(x.sizes());
+  r[1] = r[1].view(x.sizes().slice(0, x.dim() - 1));
+  if (given(residual)) r[2] = r[2].view(x.sizes());
+  else r.pop_back();
+  return r;
+}
+
+// x (..., K) int8, x_scale (...), w (N, K) int8, w_scale (N)
+Tensor int8_linear(const Tensor& x, const Tensor& xs, const Tensor& w, const Tensor& ws, OptTensor bias, int64_t out_dtype) {
+  TORCH_CHECK_TYPE(x.scalar_type() == at::kChar && w.scalar_type() == at::kChar, "x and w must be int8, got ", x.scalar_type(), " and ",
+                   w.scalar_type());
+  TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(1), "x must be (..., K), w (N, K); got ", x.sizes(), ", ", w.sizes());
+  TORCH_CHECK_VALUE(w.size(1) <= 131071, "K = ", w.size(1), " could overflow the 32-bit sums (at most 131071)");
+  const auto lead = x.sizes().slice(0, x.dim() - 1);
+  const auto vec = [&](const Tensor& t, at::IntArrayRef shape, const char* name) {
+    TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat && t.sizes() == shape, name, " must be float32 of shape ", shape, ", got ", t.scalar_type(),
+                      " ", t.sizes());
+    TORCH_CHECK(!at::GradMode::is_enabled() || !wants_grad(t), "int8_linear has no gradient (", name,
+                " requires one): call it under torch.no_grad()");
+    TORCH_CHECK_VALUE(t.device() == x.device(), name, " is on ", t.device(), ", x on ", x.device());
+  };
+  vec(xs, lead, "x_scale");
+  vec(ws, {w.size(0)}, "w_scale");
+  if (given(bias)) vec(*bias, {w.size(0)}, "bias");
+  TORCH_CHECK_VALUE(w.device() == x.device(), "w is on ", w.device(), ", x on ", x.device());
+  at::AutoDispatchBelowADInplaceOrView below;
+  int64_t M = 1;
+  for (const int64_t n : lead) M *= n;
+  std::vector<int64_t> shape(lead.begin(), lead.end());
+  shape.push_back(w.size(0));
+  return int8_mm(x.contiguous().view({M, x.size(-1)}), xs.contiguous().view({M}), w.contiguous(), ws.contiguous(),
+                 given(bias) ? std::optional<Tensor>(bias->contiguous()) : std::nullopt, out_dtype)
+      .view(shape);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(raft_amd, m) {
+  m.def("attention(Tensor q, Tensor k, Tensor v, float? scale, bool causal, Tensor? mask, Tensor? lengths, Tensor? q_offset) -> Tensor");
+  m.def("rms_norm(Tensor x, Tensor w, float eps) -> Tensor");
+  m.def("rms_norm_residual(Tensor x, Tensor w, Tensor residual, float eps) -> (Tensor, Tensor)");
+  m.def("rms_norm_int8(Tensor x, Tensor w, Tensor? residual, float eps) -> Tensor[]");
+  m.def("int8_linear(Tensor x, Tensor xs, Tensor w, Tensor ws, Tensor? bias, int out_dtype) -> Tensor");
   m.def("attn_fwd(Tensor q, Tensor k, Tensor v, float scale, bool causal, Tensor? mask, Tensor? lengths, Tensor? q_offset, bool need_lse) -> Tensor[]");
   m.def("attn_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, float scale, bool causal, Tensor? mask, Tensor? lengths, Tensor? q_offset) -> Tensor[]");
   m.def("rms_fwd(Tensor x, Tensor w, Tensor? residual, float eps, bool need_rstd) -> Tensor[]");
@@ -305,4 +510,17 @@ TORCH_LIBRARY_IMPL(raft_amd, CUDA, m) {
   m.impl("rms_fwd_int8", &rms_fwd_int8);
   m.impl("rms_bwd", &rms_bwd);
   m.impl("int8_mm", &int8_mm);
+  m.impl("attention", &attention);
+  m.impl("rms_norm", &rms_norm);
+  m.impl("rms_norm_residual", &rms_norm_residual);
+  m.impl("rms_norm_int8", &rms_norm_int8);
+  m.impl("int8_linear", &int8_linear);
+}
+
+TORCH_LIBRARY_IMPL(raft_amd, AutogradCUDA, m) {
+  m.impl("attention", &attention);
+  m.impl("rms_norm", &rms_norm);
+  m.impl("rms_norm_residual", &rms_norm_residual);
+  m.impl("rms_norm_int8", &rms_norm_int8);
+  m.impl("int8_linear", &int8_linear);
 }

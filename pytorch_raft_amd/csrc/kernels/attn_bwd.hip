@@ -3,21 +3,28 @@
 //   P = exp(scale q.k - lse), delta_i = sum_d do_id o_id, dP = do v^T, dS = P (dP - delta),
 //   dq = scale dS k, dk = scale dS^T q, dv = P^T do   (dk, dv summed over the heads of a group).
 //
-// Three kernels, none with atomics on the results (the same inputs give the same bits): row sums
-// delta; dk / dv with a workgroup per key block, walking the rows; dq with a workgroup per row
-// block, walking the keys.  Scores and dP are formed twice (7 products of L^2 D instead of 5): one
-// kernel for all three would have to add dq across key blocks, in an order that changes the sums.
-// In each kernel the score tile lies so that it is the B operand of the gradient products as it is
+// No atomics on the results (the same inputs give the same bits).  attn_prep_kernel forms delta; then
+// one launch holds two kinds of workgroups: for dk / dv, one per 128 keys walking the rows, and for dq,
+// one per 128 rows walking the keys.  Scores and dP are formed twice (7 products of L^2 D instead of
+// 5): one kind alone would have to add dq across key blocks, in an order that changes the sums.  The
+// kinds share a launch because a workgroup fills its CU (one wave per SIMD: 32 keys of dk and dv are
+// 128 accumulators): 12 x 2852 tokens make 276 workgroups of each kind for 256 CUs, and the dq ones
+// fill the second round of the others.
+// In each kind the score tile lies so that it is the B operand of the gradient products as it is
 // (attn_common.h): dk / dv own keys as columns, dq owns rows as columns.
 //
 // fp16: dS is rounded to fp16 before its product, and products of small dout with P ~ 1 / L fall
 // under fp16's range.  It is scaled by a power of two, exactly, so that its upper bound
-// 2 max|dout_i| max|v_j| maps to 2^14 (attn_delta_kernel finds the norms); P by 2^14 likewise.
+// 2 max|dout_i| max|v_j| maps to 2^14 (attn_prep_kernel finds the norms); P by 2^14 likewise.
 #include "attn_common.h"
 
 namespace attn_detail {
 
 constexpr float kP16 = 14.f;  // log2 of the fp16 scale of P
+constexpr int kPrepMax = 1024;  // most blocks of attn_prep_kernel (each leaves two norms)
+
+template <typename T>
+constexpr bool is_f16 = sizeof(T) == 2 && !__is_same(T, __bf16);
 
 template <typename T, int DP>
 struct BwdCfg {
@@ -26,11 +33,22 @@ struct BwdCfg {
   static constexpr int TILE = BT * DP * (int)sizeof(T);
 };
 
-// power of two that brings the bound of |dS| to at most 2^14 (fp16; 1 otherwise)
+// power of two that brings the bound of |dS| to at most 2^14 (fp16; 1 otherwise): a wave reads the
+// prep blocks' largest squared norms
 template <typename T>
 __device__ __forceinline__ float ds_scale(const AttnArgs& a) {
-  if constexpr (sizeof(T) == 2 && !__is_same(T, __bf16)) {
-    const float bound = 2.f * sqrtf(__uint_as_float(a.amax[0])) * sqrtf(__uint_as_float(a.amax[1]));
+  if constexpr (is_f16<T>) {
+    uint32_t m0 = 0, m1 = 0;
+    for (int i = threadIdx.x & 63; i < a.nprep; i += 64) {
+      m0 = max(m0, a.amax[2 * i]);
+      m1 = max(m1, a.amax[2 * i + 1]);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      m0 = max(m0, (uint32_t)__shfl_xor((int)m0, o, 64));
+      m1 = max(m1, (uint32_t)__shfl_xor((int)m1, o, 64));
+    }
+    const float bound = 2.f * sqrtf(__uint_as_float(m0)) * sqrtf(__uint_as_float(m1));
     if (!(bound > 0.f) || !(bound < INFINITY)) return 1.f;
     const int e = 14 - (int)ceilf(log2f(bound));
     return ldexpf(1.f, max(-100, min(100, e)));
@@ -39,69 +57,115 @@ __device__ __forceinline__ float ds_scale(const AttnArgs& a) {
   }
 }
 
-// delta of every row; fp16: also the largest squared 2-norm of a dout row and of a v row, as float
-// bits (ordered like the floats; a maximum does not depend on the order it is taken in).
-// A wave per row.  Rows R of all (b, kv head) first, then (fp16) the v rows.
+// delta of every row; fp16: also the largest squared 2-norm of a dout row and of a v row that this
+// block met, as float bits (ordered like the floats, NaN above all).  16 lanes of 8 channels a row.
 template <typename T>
-__global__ __launch_bounds__(256) void attn_delta_kernel(AttnArgs a) {
-  constexpr bool F16 = sizeof(T) == 2 && !__is_same(T, __bf16);
-  const int lane = threadIdx.x & 63;
+__global__ __launch_bounds__(256) void attn_prep_kernel(AttnArgs a) {
+  constexpr bool F16 = is_f16<T>;
+  typedef T v8 __attribute__((ext_vector_type(8)));
+  const int sub = threadIdx.x & 15, d = sub * 8;
   const int64_t R = (int64_t)a.G * a.Lq, nrow = R * a.B * a.Hkv, nv = F16 ? (int64_t)a.B * a.Hkv * a.Lk : 0;
-  uint32_t best = 0;
-  int which = -1;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (w < nrow) {
-    const int bh = (int)(w / R), row = (int)(w - (int64_t)bh * R);
-    const int b = bh / a.Hkv, hk = bh - b * a.Hkv, qi = row / a.G, h = hk * a.G + row % a.G;
-    const T* po = reinterpret_cast<const T*>(a.o) + (((int64_t)b * a.Lq + qi) * a.Hkv * a.G + h) * a.D;
-    const T* pd = reinterpret_cast<const T*>(a.dout) + b * a.d_sb + qi * a.d_sl + h * a.d_sh;
+  uint32_t best[2] = {0, 0};
+  for (int64_t w = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); w < nrow + nv; w += (int64_t)gridDim.x * 16) {
     float s = 0.f, n = 0.f;
-    for (int d = lane; d < a.D; d += 64) {
-      const float x = (float)pd[d];
-      s = fmaf(x, (float)po[d], s);
-      n = fmaf(x, x, n);
+    if (w < nrow) {
+      const int bh = (int)(w / R), row = (int)(w - (int64_t)bh * R);
+      const int b = bh / a.Hkv, hk = bh - b * a.Hkv, qi = row / a.G, h = hk * a.G + row % a.G;
+      if (d < a.D) {
+        const v8 o = *reinterpret_cast<const v8*>(reinterpret_cast<const T*>(a.o) + (((int64_t)b * a.Lq + qi) * a.Hkv * a.G + h) * a.D + d);
+        const v8 g = *reinterpret_cast<const v8*>(reinterpret_cast<const T*>(a.dout) + b * a.d_sb + qi * a.d_sl + h * a.d_sh + d);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          s = fmaf((float)g[i], (float)o[i], s);
+          n = fmaf((float)g[i], (float)g[i], n);
+        }
+      }
+    } else {
+      const int64_t e = w - nrow;
+      const int bh = (int)(e / a.Lk), j = (int)(e - (int64_t)bh * a.Lk), b = bh / a.Hkv;
+      const bool see = j < item_len(a, b) && (a.mask_mode != 1 || a.mask[b * a.m_sb + j * a.m_sk]);
+      if (see && d < a.D) {
+        const v8 v = *reinterpret_cast<const v8*>(reinterpret_cast<const T*>(a.v) + b * a.v_sb + j * a.v_sl + (bh - b * a.Hkv) * a.v_sh + d);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) n = fmaf((float)v[i], (float)v[i], n);
+      }
     }
-    s = wave_sum(s);
-    if (lane == 0) a.delta[w] = s;
+    s = raft_row16_sum(s);
+    if (w < nrow && sub == 0) a.delta[w] = s;
     if constexpr (F16) {
-      best = __float_as_uint(wave_sum(n));
-      which = 0;
+      n = raft_row16_sum(n);
+      const int k = w < nrow ? 0 : 1;
+      best[k] = max(best[k], __float_as_uint(n));
     }
-  } else if (w < nrow + nv) {
-    const int64_t e = w - nrow;
-    const int bh = (int)(e / a.Lk), j = (int)(e - (int64_t)bh * a.Lk), b = bh / a.Hkv;
-    const T* pv = reinterpret_cast<const T*>(a.v) + b * a.v_sb + j * a.v_sl + (bh - b * a.Hkv) * a.v_sh;
-    const bool see = j < item_len(a, b) && (a.mask_mode != 1 || a.mask[b * a.m_sb + j * a.m_sk]);
-    float n = 0.f;
-    for (int d = lane; see && d < a.D; d += 64) n = fmaf((float)pv[d], (float)pv[d], n);
-    best = __float_as_uint(wave_sum(n));
-    which = 1;
   }
   if constexpr (F16) {
-    if (lane == 0 && which >= 0 && best > __atomic_load_n(&a.amax[which], __ATOMIC_RELAXED))
-      atomicMax(&a.amax[which], best);
+    __shared__ uint32_t sh[2][16];
+    if (sub == 0) sh[0][threadIdx.x >> 4] = best[0], sh[1][threadIdx.x >> 4] = best[1];
+    __syncthreads();
+    if (threadIdx.x < 2) {
+      uint32_t m = 0;
+      for (int i = 0; i < 16; ++i) m = max(m, sh[threadIdx.x][i]);
+      a.amax[2 * blockIdx.x + threadIdx.x] = m;
+    }
   }
 }
 
-__global__ void attn_amax_clear_kernel(uint32_t* amax) {
-  if (threadIdx.x < 2) amax[threadIdx.x] = 0;
+// 4 consecutive channels per 4 accumulator registers: to the result, or (part) to fp32 partials
+template <typename T, int DB>
+__device__ __forceinline__ void put_grad(void* out, float* part, int64_t at, const f32x16 (&acc)[DB], float f, bool keep, int D, int hi) {
+#pragma unroll
+  for (int i = 0; i < DB; ++i)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = i * 32 + g * 8 + hi * 4;
+      if (d < D) {
+        typedef T v4 __attribute__((ext_vector_type(4)));
+        f32x4 x;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = keep ? acc[i][4 * g + k] * f : 0.f;
+        if (part) {
+          *reinterpret_cast<f32x4*>(part + at + d) = x;
+        } else {
+          v4 y;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) y[k] = (T)x[k];
+          *reinterpret_cast<v4*>(reinterpret_cast<T*>(out) + at + d) = y;
+        }
+      }
+    }
+}
+
+// workgroup -> (tile, split, batch x key head).  Without causal the blocks of a head stay on one XCD;
+// causal tiles differ in length, so they are dealt over all CUs, longest first.
+__device__ __forceinline__ bool place(const AttnArgs& a, int bid, int grid, int tiles, int nsplit, bool last_first, int& tile, int& split, int& bh) {
+  const int heads = a.B * a.Hkv;
+  const int id = a.causal ? bid : xcd_order(bid, grid);
+  if (id >= tiles * nsplit * heads) return false;
+  if (a.causal) {
+    bh = id % heads;
+    split = id / heads % nsplit;
+    tile = id / heads / nsplit;
+  } else {
+    tile = id % tiles;
+    split = id / tiles % nsplit;
+    bh = id / tiles / nsplit;
+  }
+  if (last_first) tile = tiles - 1 - tile;
+  return true;
 }
 
 // ---------------------------------------------------------------- dk, dv: a wave per 32 keys
 template <typename T, int DP, int MASK>
-__global__ __launch_bounds__(256, 1) void attn_dkv_kernel(AttnArgs a) {
+__device__ __forceinline__ void dkv_body(const AttnArgs& a, int bid, int grid, uint8_t* sm) {
   using TL = Tile<T, DP>;
   using Frag = typename TL::Frag;
-  constexpr int BT = BwdCfg<T, DP>::BT, TILE = BwdCfg<T, DP>::TILE, DB = DP / 32, DT = DP / 16;
-  constexpr bool F16 = sizeof(T) == 2 && !__is_same(T, __bf16);
-  __shared__ __attribute__((aligned(16))) uint8_t qd[2][2][TILE];
-  __shared__ __attribute__((aligned(16))) float stat[2][2][BT];  // lse, delta of the tile's rows
+  constexpr int BT = BwdCfg<T, DP>::BT, TILE = BwdCfg<T, DP>::TILE, DB = DP / 32, DT = DP / 16, NB = BT / 32;
+  constexpr bool F16 = is_f16<T>;
+  float* stat = reinterpret_cast<float*>(sm + 4 * TILE);  // [buffer][-lse, delta][row of the tile]
 
   const int R = a.G * a.Lq;
-  const int tiles = (a.Lk + 127) / 128;
-  const int id = xcd_order(blockIdx.x, gridDim.x);
-  if (id >= tiles * a.B * a.Hkv) return;
-  const int tile = id % tiles, bh = id / tiles;
+  int tile, split, bh;
+  if (!place(a, bid, grid, (a.Lk + 127) / 128, a.nsplit_kv, false, tile, split, bh)) return;
   const int b = bh / a.Hkv, hk = bh - b * a.Hkv;
   const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -112,9 +176,13 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(AttnArgs a) {
   // first query that sees any key of the workgroup / that sees all keys of the wave
   const int q_first = a.causal ? max(0, tile * 128 - off) : 0;
   const int q_full = a.causal ? tile * 128 + wave * 32 + 31 - off : 0;
-  const int64_t row_first = (int64_t)q_first * a.G;
-  const int t1 = (R + BT - 1) / BT;
-  const int t0 = tile * 128 < len ? (int)min(row_first / BT, (int64_t)t1) : t1;
+  int t1 = (R + BT - 1) / BT;
+  int t0 = tile * 128 < len ? (int)min((int64_t)q_first * a.G / BT, (int64_t)t1) : t1;
+  if (a.nsplit_kv > 1) {
+    const int per = (t1 - t0 + a.nsplit_kv - 1) / a.nsplit_kv;
+    t0 = min(t1, t0 + split * per);
+    t1 = min(t1, t0 + per);
+  }
 
   Frag kf[DT], vf[DT];
   {
@@ -137,9 +205,10 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(AttnArgs a) {
   using L = Loader<T, DP, BT, 256>;
   const uint8_t* qb = reinterpret_cast<const uint8_t*>(a.q) + (b * a.q_sb + (int64_t)hk * a.G * a.q_sh) * TL::ES;
   const uint8_t* db = reinterpret_cast<const uint8_t*>(a.dout) + (b * a.d_sb + (int64_t)hk * a.G * a.d_sh) * TL::ES;
-  const uint32_t lds = raft_lds_addr(&qd[0][0][0]) + wave * 1024;
+  const uint32_t lds = raft_lds_addr(sm) + wave * 1024;
   const float* lse = a.lse + (int64_t)bh * R;
   const float* dl = a.delta + (int64_t)bh * R;
+  const float up = ds_scale<T>(a), ds_mul = up * (F16 ? exp2f(-kP16) : 1.f);
 
   auto issue = [&](int t, int buf) {
     // rows of a tile lie at query r / G, head r % G: offsets from the tile's first query
@@ -158,51 +227,62 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(AttnArgs a) {
     }
     if (tid < 2 * BT) {
       const int r = r0 + tid % BT;
-      const float z = tid < BT ? INFINITY : 0.f;  // rows past the last: P = 0
-      stat[buf][tid / BT][tid % BT] = r < R ? (tid < BT ? lse[r] : dl[r]) : z;
+      // rows past the last: P = 0
+      stat[buf * 2 * BT + tid] = tid < BT ? (r < R ? (F16 ? kP16 : 0.f) - lse[r] : -INFINITY) : (r < R ? dl[r] * ds_mul : 0.f);
     }
   };
 
-  const float ds_mul = ds_scale<T>(a) * (F16 ? exp2f(-kP16) : 1.f);
   if (t0 < t1) issue(t0, 0);
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1;
     raft_wait_vmcnt<0>();
     __syncthreads();
     if (t + 1 < t1) issue(t + 1, buf ^ 1);
-    const uint8_t* qt = &qd[buf][0][0];
-    const uint8_t* dt = &qd[buf][1][0];
-    for (int hb = 0; hb < BT / 32; ++hb) {
-      f32x16 s = zero16(), dp = zero16();
+    const uint8_t* qt = sm + 2 * buf * TILE;
+    const uint8_t* dt = qt + TILE;
+    f32x16 s[NB], dp[NB];
+#pragma unroll
+    for (int hb = 0; hb < NB; ++hb) {
+      s[hb] = dp[hb] = zero16();
 #pragma unroll
       for (int i = 0; i < DT; ++i) {
-        s = mma(TL::rows(qt, 32 * hb + (lane & 31), i, hi), kf[i], s);
-        dp = mma(TL::rows(dt, 32 * hb + (lane & 31), i, hi), vf[i], dp);
+        s[hb] = mma(TL::rows(qt, 32 * hb + (lane & 31), i, hi), kf[i], s[hb]);
+        dp[hb] = mma(TL::rows(dt, 32 * hb + (lane & 31), i, hi), vf[i], dp[hb]);
       }
+    }
+#pragma unroll
+    for (int hb = 0; hb < NB; ++hb) {
       const bool diag = a.causal && (t * BT + 32 * hb) / a.G < q_full;
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
-        const f32x4 ls = *reinterpret_cast<const f32x4*>(&stat[buf][0][32 * hb + r4 * 8 + hi * 4]);
-        const f32x4 de = *reinterpret_cast<const f32x4*>(&stat[buf][1][32 * hb + r4 * 8 + hi * 4]);
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(stat + buf * 2 * BT + 32 * hb + r4 * 8 + hi * 4);
+        const f32x4 de = *reinterpret_cast<const f32x4*>(stat + buf * 2 * BT + BT + 32 * hb + r4 * 8 + hi * 4);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const int r = 4 * r4 + k, row = t * BT + 32 * hb + r4 * 8 + hi * 4 + k;
-          bool on = see;
-          if (diag) on = on && key <= off + row / a.G;
+          const int r = 4 * r4 + k;
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[hb][r], a.scale_log2, ls[k]));
+          s[hb][r] = p;
+          dp[hb][r] = p * (F16 ? fmaf(dp[hb][r], ds_mul, -de[k]) : dp[hb][r] - de[k]);
+        }
+      }
+      if (MASK == 2 || diag) {
+        // a hidden place adds nothing, whatever dout holds (a hidden key's column is dropped at the end)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int row = t * BT + 32 * hb + (r >> 2) * 8 + hi * 4 + (r & 3);
+          bool on = !a.causal || key <= off + row / a.G;
           if constexpr (MASK == 2) {
             const int rr = min(row, R - 1), qi = rr / a.G;
             on = on && a.mask[b * a.m_sb + (int64_t)(hk * a.G + rr - qi * a.G) * a.m_sh + (int64_t)qi * a.m_sq +
                               (int64_t)min(key, a.Lk - 1) * a.m_sk] != 0;
           }
-          float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale_log2, (F16 ? kP16 : 0.f) - ls[k]));
-          p = on ? p : 0.f;
-          s[r] = p;
-          dp[r] = on ? p * (dp[r] - de[k]) * ds_mul : 0.f;  // a hidden place adds nothing, whatever dout holds
+          s[hb][r] = on ? s[hb][r] : 0.f;
+          dp[hb][r] = on ? dp[hb][r] : 0.f;
         }
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const Frag pf = to_frag<T>(s, i), df = to_frag<T>(dp, i);
+        const Frag pf = to_frag<T>(s[hb], i), df = to_frag<T>(dp[hb], i);
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
           dv[d] = mma(TL::cols(dt, 32 * hb + 16 * i, d, lane), pf, dv[d]);
@@ -212,42 +292,23 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(AttnArgs a) {
     }
   }
   if (key >= a.Lk) return;
-  const int64_t o = (((int64_t)b * a.Lk + key) * a.Hkv + hk) * a.D;
-  const float fk = a.scale / ds_scale<T>(a), fv = F16 ? exp2f(-kP16) : 1.f;
-#pragma unroll
-  for (int i = 0; i < DB; ++i)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = i * 32 + g * 8 + hi * 4;
-      if (d < a.D) {
-        typedef T v4 __attribute__((ext_vector_type(4)));
-        v4 x, y;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          x[k] = (T)(dk[i][4 * g + k] * fk);
-          y[k] = (T)(dv[i][4 * g + k] * fv);
-        }
-        *reinterpret_cast<v4*>(reinterpret_cast<T*>(a.dk) + o + d) = x;
-        *reinterpret_cast<v4*>(reinterpret_cast<T*>(a.dv) + o + d) = y;
-      }
-    }
+  const int64_t o = (((int64_t)b * a.Lk + key) * a.Hkv + hk) * a.D, n = (int64_t)a.B * a.Lk * a.Hkv * a.D;
+  put_grad<T>(a.dk, a.nsplit_kv > 1 ? a.part + split * n : nullptr, o, dk, a.scale / up, see, a.D, hi);
+  put_grad<T>(a.dv, a.nsplit_kv > 1 ? a.part + (a.nsplit_kv + split) * n : nullptr, o, dv, F16 ? exp2f(-kP16) : 1.f, see, a.D, hi);
 }
 
 // ---------------------------------------------------------------- dq: a wave per 32 rows
 template <typename T, int DP, int MASK>
-__global__ __launch_bounds__(256, 1) void attn_dq_kernel(AttnArgs a) {
+__device__ __forceinline__ void dq_body(const AttnArgs& a, int bid, int grid, uint8_t* sm) {
   using TL = Tile<T, DP>;
   using Frag = typename TL::Frag;
-  constexpr int BK = BwdCfg<T, DP>::BT, TILE = BwdCfg<T, DP>::TILE, DB = DP / 32, DT = DP / 16;
-  constexpr bool F16 = sizeof(T) == 2 && !__is_same(T, __bf16);
-  __shared__ __attribute__((aligned(16))) uint8_t kv[2][2][TILE];
-  __shared__ __attribute__((aligned(16))) float bias[2][BK];
+  constexpr int BK = BwdCfg<T, DP>::BT, TILE = BwdCfg<T, DP>::TILE, DB = DP / 32, DT = DP / 16, NB = BK / 32;
+  constexpr bool F16 = is_f16<T>;
+  float* bias = reinterpret_cast<float*>(sm + 4 * TILE);  // [buffer][key of the tile]
 
   const int R = a.G * a.Lq;
-  const int tiles = (R + 127) / 128;
-  const int id = xcd_order(blockIdx.x, gridDim.x);
-  if (id >= tiles * a.B * a.Hkv) return;
-  const int tile = tiles - 1 - id % tiles, bh = id / tiles;
+  int tile, split, bh;
+  if (!place(a, bid, grid, (R + 127) / 128, a.nsplit_q, true, tile, split, bh)) return;
   const int b = bh / a.Hkv, hk = bh - b * a.Hkv;
   const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -259,7 +320,12 @@ __global__ __launch_bounds__(256, 1) void attn_dq_kernel(AttnArgs a) {
   const int wlim = !a.causal ? len : max(0, min(len, off + min(r0 + 31, R - 1) / a.G + 1));
   const int wmin = !a.causal ? len : max(0, min(len, off + min(r0, R - 1) / a.G + 1));
   const int blim = !a.causal ? len : max(0, min(len, off + (min(tile * 128 + 128, R) - 1) / a.G + 1));
-  const int t1 = (blim + BK - 1) / BK;
+  int t0 = 0, t1 = (blim + BK - 1) / BK;
+  if (a.nsplit_q > 1) {
+    const int per = (t1 + a.nsplit_q - 1) / a.nsplit_q;
+    t0 = min(t1, split * per);
+    t1 = min(t1, t0 + per);
+  }
 
   Frag qf[DT], df[DT];
   {
@@ -275,10 +341,9 @@ __global__ __launch_bounds__(256, 1) void attn_dq_kernel(AttnArgs a) {
       df[t] = ok && d < a.D ? *reinterpret_cast<const Frag*>(pd + d) : z;
     }
   }
-  const float lse = ok ? a.lse[(int64_t)bh * R + row] : INFINITY;
-  const float de = ok ? a.delta[(int64_t)bh * R + row] : 0.f;
-  const float sub = (F16 ? kP16 : 0.f) - lse;
-  const float ds_mul = ds_scale<T>(a) * (F16 ? exp2f(-kP16) : 1.f);
+  const float up = ds_scale<T>(a), ds_mul = up * (F16 ? exp2f(-kP16) : 1.f);
+  const float sub = ok ? (F16 ? kP16 : 0.f) - a.lse[(int64_t)bh * R + row] : -INFINITY;
+  const float de = ok ? a.delta[(int64_t)bh * R + row] * ds_mul : 0.f;
 
   f32x16 dq[DB];
 #pragma unroll
@@ -290,7 +355,7 @@ __global__ __launch_bounds__(256, 1) void attn_dq_kernel(AttnArgs a) {
   L lk, lv;
   lk.init(tid, kp, a.D * TL::ES);
   lv.init(tid, vp, a.D * TL::ES);
-  const uint32_t lds = raft_lds_addr(&kv[0][0][0]) + wave * 1024;
+  const uint32_t lds = raft_lds_addr(sm) + wave * 1024;
   const uint8_t* mk = MASK ? a.mask + b * a.m_sb + (MASK == 2 ? h * a.m_sh + (int64_t)qi * a.m_sq : 0) : nullptr;
 
   auto issue = [&](int t, int buf) {
@@ -308,75 +373,101 @@ __global__ __launch_bounds__(256, 1) void attn_dq_kernel(AttnArgs a) {
       raft_dma16(rv, lds + (2 * buf + 1) * TILE + j * 4096, see ? lv.off[j] : kOob);
     }
     if constexpr (MASK == 1) {
-      if (tid < BK) bias[buf][tid] = tid < n && mk[(int64_t)(k0 + min(tid, n - 1)) * a.m_sk] != 0 ? 0.f : -INFINITY;
+      if (tid < BK) bias[buf * BK + tid] = tid < n && mk[(int64_t)(k0 + min(tid, n - 1)) * a.m_sk] != 0 ? 0.f : -INFINITY;
     }
   };
 
-  if (t1 > 0) issue(0, 0);
-  for (int t = 0; t < t1; ++t) {
-    const int buf = t & 1, k0 = t * BK;
+  if (t0 < t1) issue(t0, 0);
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1, k0 = t * BK;
     raft_wait_vmcnt<0>();
     __syncthreads();
     if (t + 1 < t1) issue(t + 1, buf ^ 1);
     if (k0 >= wlim) continue;
-    const uint8_t* kt = &kv[buf][0][0];
-    const uint8_t* vt = &kv[buf][1][0];
-    for (int hb = 0; hb < BK / 32; ++hb) {
-      f32x16 s = zero16(), dp = zero16();
+    const uint8_t* kt = sm + 2 * buf * TILE;
+    const uint8_t* vt = kt + TILE;
+    const bool edge = MASK || k0 + BK > wmin;
+    f32x16 s[NB], dp[NB];
+#pragma unroll
+    for (int hb = 0; hb < NB; ++hb) {
+      s[hb] = dp[hb] = zero16();
 #pragma unroll
       for (int i = 0; i < DT; ++i) {
-        s = mma(TL::rows(kt, 32 * hb + (lane & 31), i, hi), qf[i], s);
-        dp = mma(TL::rows(vt, 32 * hb + (lane & 31), i, hi), df[i], dp);
+        s[hb] = mma(TL::rows(kt, 32 * hb + (lane & 31), i, hi), qf[i], s[hb]);
+        dp[hb] = mma(TL::rows(vt, 32 * hb + (lane & 31), i, hi), df[i], dp[hb]);
       }
-      const bool part = MASK || k0 + BK > wmin;
+    }
+#pragma unroll
+    for (int hb = 0; hb < NB; ++hb) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int j = 32 * hb + (r >> 2) * 8 + hi * 4 + (r & 3);
-        const float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale_log2, sub));
-        float d = p * (dp[r] - de) * ds_mul;
-        if (part) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[hb][r], a.scale_log2, sub));
+        s[hb][r] = p * (F16 ? fmaf(dp[hb][r], ds_mul, -de) : dp[hb][r] - de);
+      }
+      if (edge) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = 32 * hb + (r >> 2) * 8 + hi * 4 + (r & 3);
           bool on = j < lim - k0;
-          if constexpr (MASK == 1) on = on && bias[buf][j] == 0.f;
+          if constexpr (MASK == 1) on = on && bias[buf * BK + j] == 0.f;
           if constexpr (MASK == 2) on = on && mk[(int64_t)min(k0 + j, a.Lk - 1) * a.m_sk] != 0;
-          d = on ? d : 0.f;
+          s[hb][r] = on ? s[hb][r] : 0.f;
         }
-        s[r] = d;
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const Frag f = to_frag<T>(s, i);
+        const Frag f = to_frag<T>(s[hb], i);
 #pragma unroll
         for (int d = 0; d < DB; ++d) dq[d] = mma(TL::cols(kt, 32 * hb + 16 * i, d, lane), f, dq[d]);
       }
     }
   }
   if (!ok) return;
-  const int64_t o = (((int64_t)b * a.Lq + qi) * a.Hkv * a.G + h) * a.D;
-  const float f = a.scale / ds_scale<T>(a);
+  const int64_t o = (((int64_t)b * a.Lq + qi) * a.Hkv * a.G + h) * a.D, n = (int64_t)a.B * a.Lq * a.Hkv * a.G * a.D;
+  put_grad<T>(a.dq, a.nsplit_q > 1 ? a.part_q + split * n : nullptr, o, dq, a.scale / up, true, a.D, hi);
+}
+
+template <typename T, int DP, int MASK>
+__global__ __launch_bounds__(256, 1) void attn_bwd_kernel(AttnArgs a, int grid_kv, int grid_q) {
+  __shared__ __attribute__((aligned(16))) uint8_t sm[4 * BwdCfg<T, DP>::TILE + 4 * BwdCfg<T, DP>::BT * 4];
+  if ((int)blockIdx.x < grid_kv) dkv_body<T, DP, MASK>(a, blockIdx.x, grid_kv, sm);
+  else dq_body<T, DP, MASK>(a, blockIdx.x - grid_kv, grid_q, sm);
+}
+
+// sums of the split parts, in order: dk, dv (n_kv elements each) and dq (n_q)
+template <typename T>
+__global__ __launch_bounds__(256) void attn_grad_join_kernel(AttnArgs a, int64_t n_kv, int64_t n_q) {
+  typedef T v4 __attribute__((ext_vector_type(4)));
+  int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  const float* part = a.part;
+  void* out = a.dk;
+  int64_t n = n_kv;
+  int splits = a.nsplit_kv;
+  if (a.nsplit_kv > 1 && i < 2 * n_kv) {
+    if (i >= n_kv) part += splits * n_kv, out = a.dv, i -= n_kv;
+  } else {
+    if (a.nsplit_kv > 1) i -= 2 * n_kv;
+    part = a.part_q, out = a.dq, n = n_q, splits = a.nsplit_q;
+    if (a.nsplit_q <= 1 || i >= n_q) return;
+  }
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < splits; ++k) s += *reinterpret_cast<const f32x4*>(part + k * n + i);
+  v4 y;
 #pragma unroll
-  for (int i = 0; i < DB; ++i)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = i * 32 + g * 8 + hi * 4;
-      if (d < a.D) {
-        typedef T v4 __attribute__((ext_vector_type(4)));
-        v4 x;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = (T)(dq[i][4 * g + k] * f);
-        *reinterpret_cast<v4*>(reinterpret_cast<T*>(a.dq) + o + d) = x;
-      }
-    }
+  for (int k = 0; k < 4; ++k) y[k] = (T)s[k];
+  *reinterpret_cast<v4*>(reinterpret_cast<T*>(out) + i) = y;
 }
 
 template <typename T, int DP, int MASK>
 void bwd_launch(const AttnArgs& a, hipStream_t s) {
   const int64_t R = (int64_t)a.G * a.Lq, heads = (int64_t)a.B * a.Hkv;
-  constexpr bool F16 = sizeof(T) == 2 && !__is_same(T, __bf16);
-  if (F16) attn_amax_clear_kernel<<<1, 64, 0, s>>>(a.amax);
-  const int64_t rows = R * heads + (F16 ? heads * a.Lk : 0);
-  attn_delta_kernel<T><<<raft_cdiv(rows, 4), 256, 0, s>>>(a);
-  attn_dkv_kernel<T, DP, MASK><<<raft_cdiv((int64_t)raft_cdiv(a.Lk, 128) * heads, 8) * 8, 256, 0, s>>>(a);
-  attn_dq_kernel<T, DP, MASK><<<raft_cdiv((int64_t)raft_cdiv(R, 128) * heads, 8) * 8, 256, 0, s>>>(a);
+  attn_prep_kernel<T><<<a.nprep, 256, 0, s>>>(a);
+  const int gk = (int)raft_cdiv((int64_t)raft_cdiv(a.Lk, 128) * heads * a.nsplit_kv, 8) * 8;
+  const int gq = (int)raft_cdiv((int64_t)raft_cdiv(R, 128) * heads * a.nsplit_q, 8) * 8;
+  attn_bwd_kernel<T, DP, MASK><<<gk + gq, 256, 0, s>>>(a, gk, gq);
+  const int64_t n_kv = (int64_t)a.B * a.Lk * a.Hkv * a.D, n_q = R * heads * a.D;
+  const int64_t n = (a.nsplit_kv > 1 ? 2 * n_kv : 0) + (a.nsplit_q > 1 ? n_q : 0);
+  if (n > 0) attn_grad_join_kernel<T><<<raft_cdiv(n, 1024), 256, 0, s>>>(a, n_kv, n_q);
 }
 template <typename T, int DP>
 void bwd_mask(const AttnArgs& a, hipStream_t s) {
@@ -393,6 +484,19 @@ void bwd_dim(const AttnArgs& a, hipStream_t s) {
 }
 
 }  // namespace attn_detail
+
+void attn_bwd_plan(AttnArgs& a) {
+  const int64_t R = (int64_t)a.G * a.Lq, heads = (int64_t)a.B * a.Hkv;
+  const int64_t rows = R * heads + (a.dtype == 1 ? heads * a.Lk : 0);
+  a.nprep = (int)std::max<int64_t>(1, std::min<int64_t>((rows + 31) / 32, attn_detail::kPrepMax));
+  // few tiles over a long other side: the walk is split so that each kind has about a workgroup per
+  // CU, with at least 4 tiles of 64 each
+  const auto split = [](int64_t blocks, int64_t walk) {
+    return (int)std::max<int64_t>(1, std::min<int64_t>({256 / std::max<int64_t>(blocks, 1), walk / 256, 32}));
+  };
+  a.nsplit_kv = split((int64_t)raft_cdiv(a.Lk, 128) * heads, R);
+  a.nsplit_q = split((int64_t)raft_cdiv(R, 128) * heads, a.Lk);
+}
 
 void launch_attn_bwd(const AttnArgs& a, hipStream_t s) {
   if (a.dtype == 0) attn_detail::bwd_dim<__bf16>(a, s);

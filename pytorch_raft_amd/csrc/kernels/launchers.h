@@ -476,11 +476,15 @@ struct AttnArgs {
   const void* dout;       // (B, Lq, H, D), strides d_*
   int64_t d_sb, d_sl, d_sh;
   float* delta;
-  uint32_t* amax;         // fp16 only: largest |dout row| and |v row| (2-norms, as float bits)
+  uint32_t* amax;         // fp16 only: (nprep, 2) largest squared norms of a dout row and a v row (float bits)
+  int nprep;              // blocks of the first launch
+  int nsplit_kv, nsplit_q;  // walks of the dk / dv and dq workgroups split into parts (attn_bwd_plan)
+  float* part_q;          // (nsplit_q, dq); part holds (2, nsplit_kv, dk) then
   void *dq, *dk, *dv;     // contiguous (B, L, heads, D)
 };
 int attn_splits(const AttnArgs& a);
 void launch_attn_fwd(const AttnArgs& a, hipStream_t s);
+void attn_bwd_plan(AttnArgs& a);  // nprep, nsplit_kv, nsplit_q
 void launch_attn_bwd(const AttnArgs& a, hipStream_t s);
 
 // ---- root-mean-square norm (rms_norm.hip): rows x C, contiguous; C <= 16384

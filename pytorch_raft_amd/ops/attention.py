@@ -24,7 +24,6 @@ splits the keys.
 The all-pairs correlation (ops/corr.py) is the same product of two feature maps without the softmax.
 """
 import torch
-import torch.nn.functional as F
 
 from . import _ext
 
@@ -58,24 +57,6 @@ def torch_attention(q, k, v, scale=None, causal=False, mask=None, lengths=None, 
     return torch.matmul(p, v.transpose(1, 2).contiguous()).transpose(1, 2)
 
 
-class _Attention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, scale, causal, mask, lengths, q_offset):
-        need = any(ctx.needs_input_grad[:3])
-        out, lse = _ext.ops().attn_fwd(q, k, v, scale, causal, mask, lengths, q_offset, need)
-        if need:
-            ctx.save_for_backward(q, k, v, out, lse, mask, lengths, q_offset)
-            ctx.p = (scale, causal)
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout):
-        q, k, v, out, lse, mask, lengths, q_offset = ctx.saved_tensors
-        dq, dk, dv = _ext.ops().attn_bwd(dout, q, k, v, out, lse, *ctx.p, mask, lengths, q_offset)
-        return dq, dk, dv, None, None, None, None, None
-
-
 def _check(q, k, v, scale, mask, lengths, q_offset):
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
         raise ValueError('q must be (B, Lq, H, D), k and v (B, Lk, Hkv, D); got %s, %s, %s'
@@ -105,19 +86,9 @@ def _check(q, k, v, scale, mask, lengths, q_offset):
 
 
 def attention(q, k, v, scale=None, causal=False, mask=None, lengths=None, q_offset=None, impl='auto'):
+    if impl != 'torch' and _ext.device_ok(q) and _ext.gpu_path_enabled(required=(impl == 'hip')):
+        # (checks, padding and the autograd node are the operator's own: csrc/bindings_tokens.cpp)
+        return _ext.ops().attention(q, k, v, scale, causal, mask, lengths, q_offset)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     _check(q, k, v, scale, mask, lengths, q_offset)
-    if impl != 'torch' and _ext.device_ok(q) and _ext.gpu_path_enabled(required=(impl == 'hip')):
-        if q.dtype not in (torch.bfloat16, torch.float16, torch.float32):
-            raise TypeError('attention runs in bf16, fp16 and fp32, got %s' % q.dtype)
-        d = q.shape[-1]
-        pad = -d % 8
-        if pad:
-            q, k, v = (F.pad(t, (0, pad)) for t in (q, k, v))
-        if mask is not None:
-            mask = mask.expand(q.shape[0], q.shape[2], q.shape[1], k.shape[1])
-        out = _Attention.apply(q, k, v, scale, bool(causal), mask,
-                               None if lengths is None else lengths.contiguous(),
-                               None if q_offset is None else q_offset.contiguous())
-        return out[..., :d] if pad else out
     return torch_attention(q, k, v, scale, causal, mask, lengths, q_offset)

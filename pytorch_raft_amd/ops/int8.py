@@ -33,6 +33,11 @@ def torch_int8_linear(x, x_scale, w, w_scale, bias=None, out_dtype=torch.bfloat1
 
 
 def int8_linear(x, x_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16, impl='auto'):
+    if impl != 'torch' and _ext.device_ok(x) and _ext.gpu_path_enabled(required=(impl == 'hip')):
+        # (the checks are the operator's own: csrc/bindings_tokens.cpp)
+        if out_dtype not in _CODES:
+            raise TypeError('out_dtype must be bfloat16, float16 or float32, got %s' % out_dtype)
+        return _ext.ops().int8_linear(x, x_scale, w, w_scale, bias, _CODES[out_dtype])
     if x.dtype != torch.int8 or w.dtype != torch.int8:
         raise TypeError('x and w must be int8, got %s and %s' % (x.dtype, w.dtype))
     if out_dtype not in _CODES:
@@ -52,8 +57,4 @@ def int8_linear(x, x_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16, imp
     for name, t in (('x_scale', x_scale), ('w', w), ('w_scale', w_scale), ('bias', bias)):
         if t is not None and t.device != x.device:
             raise ValueError('%s is on %s, x on %s' % (name, t.device, x.device))
-    if impl != 'torch' and _ext.device_ok(x) and _ext.gpu_path_enabled(required=(impl == 'hip')):
-        out = _ext.ops().int8_mm(x.reshape(x.shape[:-1].numel(), k).contiguous(), x_scale.reshape(-1).contiguous(), w.contiguous(),
-                                 w_scale.contiguous(), None if bias is None else bias.contiguous(), _CODES[out_dtype])
-        return out.view(*x.shape[:-1], n)
     return torch_int8_linear(x, x_scale, w, w_scale, bias, out_dtype)

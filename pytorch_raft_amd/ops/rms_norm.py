@@ -40,28 +40,6 @@ def torch_rms_norm_int8(x, weight, residual=None, eps=1e-6):
     return q.nan_to_num(0.).to(torch.int8), (top / 127).squeeze(-1), None if residual is None else h
 
 
-class _RmsNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, residual, eps):
-        need = any(ctx.needs_input_grad[:3])
-        y, h, rstd = _ext.ops().rms_fwd(x, weight, residual, eps, need)
-        ctx.set_materialize_grads(False)
-        ctx.residual = residual is not None
-        if need:
-            ctx.save_for_backward(h if ctx.residual else x, weight, rstd)
-        return (y, h) if ctx.residual else y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy, dh=None):
-        h, weight, rstd = ctx.saved_tensors
-        dh = None if dh is None else dh.contiguous()
-        if dy is None:
-            return dh, None, dh, None
-        dx, dw = _ext.ops().rms_bwd(dy.contiguous(), dh, h, weight, rstd)
-        return dx, dw, dx if ctx.residual else None, None
-
-
 def _check(x, weight, residual, eps):
     if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_CHANNELS:
         raise ValueError('x must be (..., C) with 1 .. %d channels, got %s' % (MAX_CHANNELS, tuple(x.shape)))
@@ -80,30 +58,24 @@ def _check(x, weight, residual, eps):
 
 
 def _on_gpu(x, impl):
-    if impl == 'torch' or not _ext.device_ok(x) or not _ext.gpu_path_enabled(required=(impl == 'hip')):
-        return False
-    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
-        raise TypeError('rms_norm runs in bf16, fp16 and fp32, got %s' % x.dtype)
-    return True
+    return impl != 'torch' and _ext.device_ok(x) and _ext.gpu_path_enabled(required=(impl == 'hip'))
 
 
 def rms_norm(x, weight, residual=None, eps=1e-6, impl='auto'):
+    if _on_gpu(x, impl):
+        # (checks and the autograd node are the operator's own: csrc/bindings_tokens.cpp)
+        if residual is None:
+            return _ext.ops().rms_norm(x, weight, eps)
+        return _ext.ops().rms_norm_residual(x, weight, residual, eps)
     _check(x, weight, residual, eps)
-    if not _on_gpu(x, impl):
-        return torch_rms_norm(x, weight, residual, eps)
-    c = x.shape[-1]
-    out = _RmsNorm.apply(x.reshape(-1, c).contiguous(), weight.contiguous(),
-                         None if residual is None else residual.reshape(-1, c).contiguous(), float(eps))
-    return out.view(x.shape) if residual is None else tuple(t.view(x.shape) for t in out)
+    return torch_rms_norm(x, weight, residual, eps)
 
 
 def rms_norm_int8(x, weight, residual=None, eps=1e-6, impl='auto'):
+    if _on_gpu(x, impl):
+        out = _ext.ops().rms_norm_int8(x, weight, residual, eps)
+        return tuple(out) if residual is not None else (*out, None)
     _check(x, weight, residual, eps)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         raise RuntimeError('rms_norm_int8 has no gradient: call it under torch.no_grad()')
-    if not _on_gpu(x, impl):
-        return torch_rms_norm_int8(x, weight, residual, eps)
-    c = x.shape[-1]
-    q, scale, h = _ext.ops().rms_fwd_int8(x.reshape(-1, c).contiguous(), weight.contiguous(),
-                                          None if residual is None else residual.reshape(-1, c).contiguous(), float(eps))
-    return q.view(x.shape), scale.view(x.shape[:-1]), None if residual is None else h.view(x.shape)
+    return torch_rms_norm_int8(x, weight, residual, eps)
