@@ -123,7 +123,7 @@ std::vector<Tensor> attn_fwd(const Tensor& q0, const Tensor& k0, const Tensor& v
   Tensor lse = need_lse ? at::empty({a.B, a.Hkv, R}, f32) : at::empty({0}, f32);
   a.o = out.data_ptr();
   a.lse = need_lse ? lse.data_ptr<float>() : nullptr;
-  a.nsplit = attn_splits(a);
+  attn_fwd_plan(a);
   Tensor part;
   if (a.nsplit > 1) {
     const int64_t n = (int64_t)a.B * a.Hkv * a.nsplit * R;

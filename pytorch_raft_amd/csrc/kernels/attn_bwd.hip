@@ -33,6 +33,10 @@ struct BwdCfg {
   static constexpr int TILE = BT * DP * (int)sizeof(T);
 };
 
+// waves per SIMD that the registers allow
+template <typename T, int DP>
+constexpr int bwd_waves = DP * (int)sizeof(T) > 128 ? 1 : 2;
+
 // power of two that brings the bound of |dS| to at most 2^14 (fp16; 1 otherwise): a wave reads the
 // prep blocks' largest squared norms
 template <typename T>
@@ -110,6 +114,23 @@ __global__ __launch_bounds__(256) void attn_prep_kernel(AttnArgs a) {
   }
 }
 
+template <bool V>
+struct Bool {
+  static constexpr bool value = V;
+};
+
+// pins the schedule of a run of N matrix instructions: READS LDS reads after each.  (Pinning vector
+// instructions between them as well measured slower: 253 us with 0, 267 with 4, 290 with 6 each on the
+// backward of 12 x 2852 tokens with a head of 128, 274 without any pin.)
+template <int N, int READS>
+__device__ __forceinline__ void pin() {
+  if constexpr (N > 0) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    pin<N - 1, READS>();
+  }
+}
+
 // 4 consecutive channels per 4 accumulator registers: to the result, or (part) to fp32 partials
 template <typename T, int DB>
 __device__ __forceinline__ void put_grad(void* out, float* part, int64_t at, const f32x16 (&acc)[DB], float f, bool keep, int D, int hi) {
@@ -135,33 +156,15 @@ __device__ __forceinline__ void put_grad(void* out, float* part, int64_t at, con
     }
 }
 
-// workgroup -> (tile, split, batch x key head).  Without causal the blocks of a head stay on one XCD;
-// causal tiles differ in length, so they are dealt over all CUs, longest first.
-__device__ __forceinline__ bool place(const AttnArgs& a, int bid, int grid, int tiles, int nsplit, bool last_first, int& tile, int& split, int& bh) {
-  const int heads = a.B * a.Hkv;
-  const int id = a.causal ? bid : xcd_order(bid, grid);
-  if (id >= tiles * nsplit * heads) return false;
-  if (a.causal) {
-    bh = id % heads;
-    split = id / heads % nsplit;
-    tile = id / heads / nsplit;
-  } else {
-    tile = id % tiles;
-    split = id / tiles % nsplit;
-    bh = id / tiles / nsplit;
-  }
-  if (last_first) tile = tiles - 1 - tile;
-  return true;
-}
-
 // ---------------------------------------------------------------- dk, dv: a wave per 32 keys
 template <typename T, int DP, int MASK>
 __device__ __forceinline__ void dkv_body(const AttnArgs& a, int bid, int grid, uint8_t* sm) {
   using TL = Tile<T, DP>;
   using Frag = typename TL::Frag;
   constexpr int BT = BwdCfg<T, DP>::BT, TILE = BwdCfg<T, DP>::TILE, DB = DP / 32, DT = DP / 16, NB = BT / 32;
+  constexpr bool AHEAD = sizeof(T) == 2;  // fp32: the products take 16 times as long, and fragments twice the registers
   constexpr bool F16 = is_f16<T>;
-  float* stat = reinterpret_cast<float*>(sm + 4 * TILE);  // [buffer][-lse, delta][row of the tile]
+  float* stat = reinterpret_cast<float*>(sm + 6 * TILE);  // [buffer][-lse, delta][row of the tile]
 
   const int R = a.G * a.Lq;
   int tile, split, bh;
@@ -173,9 +176,9 @@ __device__ __forceinline__ void dkv_body(const AttnArgs& a, int bid, int grid, u
   const int key = tile * 128 + wave * 32 + (lane & 31);
   bool see = key < len;
   if constexpr (MASK == 1) see = see && a.mask[b * a.m_sb + (int64_t)min(key, a.Lk - 1) * a.m_sk] != 0;
-  // first query that sees any key of the workgroup / that sees all keys of the wave
+  // first query that sees any key of the workgroup / that sees all of them
   const int q_first = a.causal ? max(0, tile * 128 - off) : 0;
-  const int q_full = a.causal ? tile * 128 + wave * 32 + 31 - off : 0;
+  const int q_full = a.causal ? tile * 128 + 127 - off : 0;
   int t1 = (R + BT - 1) / BT;
   int t0 = tile * 128 < len ? (int)min((int64_t)q_first * a.G / BT, (int64_t)t1) : t1;
   if (a.nsplit_kv > 1) {
@@ -206,90 +209,161 @@ __device__ __forceinline__ void dkv_body(const AttnArgs& a, int bid, int grid, u
   const uint8_t* qb = reinterpret_cast<const uint8_t*>(a.q) + (b * a.q_sb + (int64_t)hk * a.G * a.q_sh) * TL::ES;
   const uint8_t* db = reinterpret_cast<const uint8_t*>(a.dout) + (b * a.d_sb + (int64_t)hk * a.G * a.d_sh) * TL::ES;
   const uint32_t lds = raft_lds_addr(sm) + wave * 1024;
+  const uint32_t qrow = TL::rows_base(raft_lds_addr(sm), lane), qcol = TL::cols_base(raft_lds_addr(sm), lane);
   const float* lse = a.lse + (int64_t)bh * R;
   const float* dl = a.delta + (int64_t)bh * R;
   const float up = ds_scale<T>(a), ds_mul = up * (F16 ? exp2f(-kP16) : 1.f);
 
-  auto issue = [&](int t, int buf) {
-    // rows of a tile lie at query r / G, head r % G: offsets from the tile's first query
-    const int r0 = t * BT, q0 = r0 / a.G;
-    const rsrc_t rq = rsrc_of(qb + (int64_t)q0 * a.q_sl * TL::ES, 0x7fffffffu);
-    const rsrc_t rd = rsrc_of(db + (int64_t)q0 * a.d_sl * TL::ES, 0x7fffffffu);
+  // Rows of a tile lie at query r / G, head r % G: byte offsets from the tile's first query.  Where G
+  // divides the tile (every G up to 64 but 3, 5, 6, 7, ...) they are the same for all tiles.
+  const bool even = BT % a.G == 0;
+  uint32_t oq[L::PER], od[L::PER];
+  auto offsets = [&](int r0, int q0) {
 #pragma unroll
     for (int j = 0; j < L::PER; ++j) {
       const int r = r0 + L::row_of(tid, j), c = L::chunk_of(tid, j) * 16;
       const int qi = r / a.G, g = r - qi * a.G;
-      const bool ok = r < R && c < a.D * TL::ES;
-      const uint32_t oq = (uint32_t)(((qi - q0) * a.q_sl + g * a.q_sh) * TL::ES) + c;
-      const uint32_t od = (uint32_t)(((qi - q0) * a.d_sl + g * a.d_sh) * TL::ES) + c;
-      raft_dma16(rq, lds + (2 * buf) * TILE + j * 4096, ok ? oq : kOob);
-      raft_dma16(rd, lds + (2 * buf + 1) * TILE + j * 4096, ok ? od : kOob);
+      oq[j] = c < a.D * TL::ES ? (uint32_t)(((qi - q0) * a.q_sl + g * a.q_sh) * TL::ES) + c : kOob;
+      od[j] = c < a.D * TL::ES ? (uint32_t)(((qi - q0) * a.d_sl + g * a.d_sh) * TL::ES) + c : kOob;
+    }
+  };
+  offsets(0, 0);
+  auto issue = [&](int t, uint32_t buf, int sbuf) {
+    const int r0 = t * BT, q0 = r0 / a.G;
+    const rsrc_t rq = rsrc_of(qb + (int64_t)q0 * a.q_sl * TL::ES, 0x7fffffffu);
+    const rsrc_t rd = rsrc_of(db + (int64_t)q0 * a.d_sl * TL::ES, 0x7fffffffu);
+    if (!even) offsets(r0, q0);
+#pragma unroll
+    for (int j = 0; j < L::PER; ++j) {
+      const bool ok = r0 + L::row_of(tid, j) < R;
+      raft_dma16(rq, lds + buf + j * 4096, ok ? oq[j] : kOob);
+      raft_dma16(rd, lds + buf + TILE + j * 4096, ok ? od[j] : kOob);
     }
     if (tid < 2 * BT) {
       const int r = r0 + tid % BT;
       // rows past the last: P = 0
-      stat[buf * 2 * BT + tid] = tid < BT ? (r < R ? (F16 ? kP16 : 0.f) - lse[r] : -INFINITY) : (r < R ? dl[r] * ds_mul : 0.f);
+      stat[sbuf + tid] = tid < BT ? (r < R ? (F16 ? kP16 : 0.f) - lse[r] : -INFINITY) : (r < R ? dl[r] * ds_mul : 0.f);
     }
   };
 
-  if (t0 < t1) issue(t0, 0);
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
+  // A tile of two 32-row blocks (16-bit types): scores and dP of both, exponentials of the first beside
+  // the products of the second, exponentials of the second beside the gradients of the first, gradients
+  // of the second; the fragments of each phase are read during the one before.  The order is pinned:
+  // left alone, the compiler puts an LDS read right before its product and waits for it there.
+  Frag fq[DT], fd[DT], cd[2][DB], cq[2][DB];
+  auto load_rows = [&](uint32_t at, int hb) {
+#pragma unroll
+    for (int i = 0; i < DT; ++i) {
+      fq[i] = TL::rows(qrow + at, hb, i);
+      fd[i] = TL::rows(qrow + at + TILE, hb, i);
+    }
+  };
+  auto load_cols = [&](uint32_t at, int hb) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        cd[i][d] = TL::cols(qcol + at + TILE, 32 * hb + 16 * i, d);
+        cq[i][d] = TL::cols(qcol + at, 32 * hb + 16 * i, d);
+      }
+  };
+  auto products = [&](f32x16& s, f32x16& dp, uint32_t at, int hb) {
+    s = dp = zero16();
+#pragma unroll
+    for (int i = 0; i < DT; ++i) {
+      s = mma(AHEAD ? fq[i] : TL::rows(qrow + at, hb, i), kf[i], s);
+      dp = mma(AHEAD ? fd[i] : TL::rows(qrow + at + TILE, hb, i), vf[i], dp);
+    }
+  };
+  auto weights = [&](auto edge, f32x16& s, f32x16& dp, int row0, const float* st) {
+#pragma unroll
+    for (int r4 = 0; r4 < 4; ++r4) {
+      const f32x4 ls = *reinterpret_cast<const f32x4*>(st + r4 * 8 + hi * 4);
+      const f32x4 de = *reinterpret_cast<const f32x4*>(st + BT + r4 * 8 + hi * 4);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int r = 4 * r4 + k;
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale_log2, ls[k]));
+        s[r] = p;
+        dp[r] = p * (F16 ? fmaf(dp[r], ds_mul, -de[k]) : dp[r] - de[k]);
+      }
+    }
+    if constexpr (decltype(edge)::value) {
+      // a hidden place adds nothing, whatever dout holds (a hidden key's column is dropped at the end)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int row = row0 + (r >> 2) * 8 + hi * 4 + (r & 3);
+        bool on = !a.causal || key <= off + row / a.G;
+        if constexpr (MASK == 2) {
+          const int rr = min(row, R - 1), qi = rr / a.G;
+          on = on && a.mask[b * a.m_sb + (int64_t)(hk * a.G + rr - qi * a.G) * a.m_sh + (int64_t)qi * a.m_sq +
+                            (int64_t)min(key, a.Lk - 1) * a.m_sk] != 0;
+        }
+        s[r] = on ? s[r] : 0.f;
+        dp[r] = on ? dp[r] : 0.f;
+      }
+    }
+  };
+  auto gradients = [&](const f32x16& s, const f32x16& dp, uint32_t at, int hb) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const Frag pf = to_frag<T>(s, i), df = to_frag<T>(dp, i);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        dv[d] = mma(AHEAD ? cd[i][d] : TL::cols(qcol + at + TILE, 32 * hb + 16 * i, d), pf, dv[d]);
+        dk[d] = mma(AHEAD ? cq[i][d] : TL::cols(qcol + at, 32 * hb + 16 * i, d), df, dk[d]);
+      }
+    }
+  };
+  auto walk = [&](auto edge, int row0, uint32_t at, const float* st, uint32_t at_next) {
+    if constexpr (NB == 2) {
+      f32x16 s0, p0, s1, p1;
+      products(s0, p0, at, 0);
+      load_rows(at, 1);
+      pin<2 * DT, 1>();
+      products(s1, p1, at, 1);
+      load_cols(at, 0);
+      weights(edge, s0, p0, row0, st);
+      pin<2 * DT, 2>();
+      gradients(s0, p0, at, 0);
+      load_cols(at, 1);
+      weights(edge, s1, p1, row0 + 32, st + 32);
+      pin<2 * DT, 2>();
+      gradients(s1, p1, at, 1);
+      load_rows(at_next, 0);
+      pin<2 * DT, 1>();
+    } else {
+      f32x16 s, dp;
+      products(s, dp, at, 0);
+      weights(edge, s, dp, row0, st);
+      gradients(s, dp, at, 0);
+    }
+  };
+  // three buffers: tile t + 1 has landed when tile t begins, for the last block's look ahead
+  uint32_t b0 = 0, b1 = 2 * TILE, b2 = 4 * TILE;
+  int s0 = 0, s1 = 2 * BT, s2 = 4 * BT;
+  auto turn = [&](auto edge, int t) {
+    raft_wait_vmcnt<0>();
+    __syncthreads();  // tile t + 1 has landed for all waves, and all have left tile t - 1
+    if (t + 2 < t1) issue(t + 2, b2, s2);
+    walk(edge, t * BT, b0, stat + s0, b1);
+    const uint32_t x = b0;
+    b0 = b1, b1 = b2, b2 = x;
+    const int y = s0;
+    s0 = s1, s1 = s2, s2 = y;
+  };
+  if (t0 < t1) {
+    issue(t0, b0, s0);
+    if (t0 + 1 < t1) issue(t0 + 1, b1, s1);
     raft_wait_vmcnt<0>();
     __syncthreads();
-    if (t + 1 < t1) issue(t + 1, buf ^ 1);
-    const uint8_t* qt = sm + 2 * buf * TILE;
-    const uint8_t* dt = qt + TILE;
-    f32x16 s[NB], dp[NB];
-#pragma unroll
-    for (int hb = 0; hb < NB; ++hb) {
-      s[hb] = dp[hb] = zero16();
-#pragma unroll
-      for (int i = 0; i < DT; ++i) {
-        s[hb] = mma(TL::rows(qt, 32 * hb + (lane & 31), i, hi), kf[i], s[hb]);
-        dp[hb] = mma(TL::rows(dt, 32 * hb + (lane & 31), i, hi), vf[i], dp[hb]);
-      }
-    }
-#pragma unroll
-    for (int hb = 0; hb < NB; ++hb) {
-      const bool diag = a.causal && (t * BT + 32 * hb) / a.G < q_full;
-#pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4) {
-        const f32x4 ls = *reinterpret_cast<const f32x4*>(stat + buf * 2 * BT + 32 * hb + r4 * 8 + hi * 4);
-        const f32x4 de = *reinterpret_cast<const f32x4*>(stat + buf * 2 * BT + BT + 32 * hb + r4 * 8 + hi * 4);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int r = 4 * r4 + k;
-          const float p = __builtin_amdgcn_exp2f(fmaf(s[hb][r], a.scale_log2, ls[k]));
-          s[hb][r] = p;
-          dp[hb][r] = p * (F16 ? fmaf(dp[hb][r], ds_mul, -de[k]) : dp[hb][r] - de[k]);
-        }
-      }
-      if (MASK == 2 || diag) {
-        // a hidden place adds nothing, whatever dout holds (a hidden key's column is dropped at the end)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int row = t * BT + 32 * hb + (r >> 2) * 8 + hi * 4 + (r & 3);
-          bool on = !a.causal || key <= off + row / a.G;
-          if constexpr (MASK == 2) {
-            const int rr = min(row, R - 1), qi = rr / a.G;
-            on = on && a.mask[b * a.m_sb + (int64_t)(hk * a.G + rr - qi * a.G) * a.m_sh + (int64_t)qi * a.m_sq +
-                              (int64_t)min(key, a.Lk - 1) * a.m_sk] != 0;
-          }
-          s[hb][r] = on ? s[hb][r] : 0.f;
-          dp[hb][r] = on ? dp[hb][r] : 0.f;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const Frag pf = to_frag<T>(s[hb], i), df = to_frag<T>(dp[hb], i);
-#pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          dv[d] = mma(TL::cols(dt, 32 * hb + 16 * i, d, lane), pf, dv[d]);
-          dk[d] = mma(TL::cols(qt, 32 * hb + 16 * i, d, lane), df, dk[d]);
-        }
-      }
-    }
+    if constexpr (AHEAD) load_rows(b0, 0);
+    int t = t0;
+    // tiles with rows that miss some of the wave's keys come first
+    const int te = MASK == 2 ? t1 : a.causal ? max(t0, min(t1, (int)(((int64_t)max(q_full, 0) * a.G + BT - 1) / BT))) : t0;
+    for (; t < te; ++t) turn(Bool<true>{}, t);
+    if constexpr (MASK != 2)
+      for (; t < t1; ++t) turn(Bool<false>{}, t);
   }
   if (key >= a.Lk) return;
   const int64_t o = (((int64_t)b * a.Lk + key) * a.Hkv + hk) * a.D, n = (int64_t)a.B * a.Lk * a.Hkv * a.D;
@@ -303,8 +377,9 @@ __device__ __forceinline__ void dq_body(const AttnArgs& a, int bid, int grid, ui
   using TL = Tile<T, DP>;
   using Frag = typename TL::Frag;
   constexpr int BK = BwdCfg<T, DP>::BT, TILE = BwdCfg<T, DP>::TILE, DB = DP / 32, DT = DP / 16, NB = BK / 32;
+  constexpr bool AHEAD = sizeof(T) == 2;
   constexpr bool F16 = is_f16<T>;
-  float* bias = reinterpret_cast<float*>(sm + 4 * TILE);  // [buffer][key of the tile]
+  float* bias = reinterpret_cast<float*>(sm + 6 * TILE);  // [buffer][key of the tile]
 
   const int R = a.G * a.Lq;
   int tile, split, bh;
@@ -317,9 +392,9 @@ __device__ __forceinline__ void dq_body(const AttnArgs& a, int bid, int grid, ui
   const int qi = rc / a.G, h = hk * a.G + rc - qi * a.G;
   const int len = item_len(a, b), off = item_off(a, b);
   const int lim = a.causal ? max(0, min(len, off + qi + 1)) : len;
-  const int wlim = !a.causal ? len : max(0, min(len, off + min(r0 + 31, R - 1) / a.G + 1));
-  const int wmin = !a.causal ? len : max(0, min(len, off + min(r0, R - 1) / a.G + 1));
+  // keys that the last / first row of the workgroup sees
   const int blim = !a.causal ? len : max(0, min(len, off + (min(tile * 128 + 128, R) - 1) / a.G + 1));
+  const int bmin = !a.causal ? len : max(0, min(len, off + min(tile * 128, R - 1) / a.G + 1));
   int t0 = 0, t1 = (blim + BK - 1) / BK;
   if (a.nsplit_q > 1) {
     const int per = (t1 + a.nsplit_q - 1) / a.nsplit_q;
@@ -356,9 +431,10 @@ __device__ __forceinline__ void dq_body(const AttnArgs& a, int bid, int grid, ui
   lk.init(tid, kp, a.D * TL::ES);
   lv.init(tid, vp, a.D * TL::ES);
   const uint32_t lds = raft_lds_addr(sm) + wave * 1024;
+  const uint32_t krow = TL::rows_base(raft_lds_addr(sm), lane), kcol = TL::cols_base(raft_lds_addr(sm), lane);
   const uint8_t* mk = MASK ? a.mask + b * a.m_sb + (MASK == 2 ? h * a.m_sh + (int64_t)qi * a.m_sq : 0) : nullptr;
 
-  auto issue = [&](int t, int buf) {
+  auto issue = [&](int t, uint32_t buf, int sbuf) {
     const int k0 = t * BK, n = min(BK, len - k0);
     const rsrc_t rk = rows_rsrc(kb + (int64_t)k0 * kp, n, kp, a.D * TL::ES);
     const rsrc_t rv = rows_rsrc(vb + (int64_t)k0 * vp, n, vp, a.D * TL::ES);
@@ -369,58 +445,108 @@ __device__ __forceinline__ void dq_body(const AttnArgs& a, int bid, int grid, ui
         const int r = L::row_of(tid, j);
         see = r < n && mk[(int64_t)(k0 + min(r, n - 1)) * a.m_sk] != 0;
       }
-      raft_dma16(rk, lds + (2 * buf) * TILE + j * 4096, see ? lk.off[j] : kOob);
-      raft_dma16(rv, lds + (2 * buf + 1) * TILE + j * 4096, see ? lv.off[j] : kOob);
+      raft_dma16(rk, lds + buf + j * 4096, see ? lk.off[j] : kOob);
+      raft_dma16(rv, lds + buf + TILE + j * 4096, see ? lv.off[j] : kOob);
     }
     if constexpr (MASK == 1) {
-      if (tid < BK) bias[buf * BK + tid] = tid < n && mk[(int64_t)(k0 + min(tid, n - 1)) * a.m_sk] != 0 ? 0.f : -INFINITY;
+      if (tid < BK) bias[sbuf + tid] = tid < n && mk[(int64_t)(k0 + min(tid, n - 1)) * a.m_sk] != 0 ? 0.f : -INFINITY;
     }
   };
 
-  if (t0 < t1) issue(t0, 0);
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1, k0 = t * BK;
-    raft_wait_vmcnt<0>();
-    __syncthreads();
-    if (t + 1 < t1) issue(t + 1, buf ^ 1);
-    if (k0 >= wlim) continue;
-    const uint8_t* kt = sm + 2 * buf * TILE;
-    const uint8_t* vt = kt + TILE;
-    const bool edge = MASK || k0 + BK > wmin;
-    f32x16 s[NB], dp[NB];
+  // (the dk / dv kind's pattern with keys and rows exchanged)
+  Frag fk[DT], fv[DT], ck[2][DB];
+  auto load_rows = [&](uint32_t at, int hb) {
 #pragma unroll
-    for (int hb = 0; hb < NB; ++hb) {
-      s[hb] = dp[hb] = zero16();
-#pragma unroll
-      for (int i = 0; i < DT; ++i) {
-        s[hb] = mma(TL::rows(kt, 32 * hb + (lane & 31), i, hi), qf[i], s[hb]);
-        dp[hb] = mma(TL::rows(vt, 32 * hb + (lane & 31), i, hi), df[i], dp[hb]);
-      }
+    for (int i = 0; i < DT; ++i) {
+      fk[i] = TL::rows(krow + at, hb, i);
+      fv[i] = TL::rows(krow + at + TILE, hb, i);
     }
+  };
+  auto load_cols = [&](uint32_t at, int hb) {
 #pragma unroll
-    for (int hb = 0; hb < NB; ++hb) {
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int d = 0; d < DB; ++d) ck[i][d] = TL::cols(kcol + at, 32 * hb + 16 * i, d);
+  };
+  auto products = [&](f32x16& s, f32x16& dp, uint32_t at, int hb) {
+    s = dp = zero16();
+#pragma unroll
+    for (int i = 0; i < DT; ++i) {
+      s = mma(AHEAD ? fk[i] : TL::rows(krow + at, hb, i), qf[i], s);
+      dp = mma(AHEAD ? fv[i] : TL::rows(krow + at + TILE, hb, i), df[i], dp);
+    }
+  };
+  auto weights = [&](auto edge, f32x16& s, const f32x16& dp, int k0, const float* bs) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale_log2, sub));
+      s[r] = p * (F16 ? fmaf(dp[r], ds_mul, -de) : dp[r] - de);
+    }
+    if constexpr (decltype(edge)::value) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(s[hb][r], a.scale_log2, sub));
-        s[hb][r] = p * (F16 ? fmaf(dp[hb][r], ds_mul, -de) : dp[hb][r] - de);
-      }
-      if (edge) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j = 32 * hb + (r >> 2) * 8 + hi * 4 + (r & 3);
-          bool on = j < lim - k0;
-          if constexpr (MASK == 1) on = on && bias[buf * BK + j] == 0.f;
-          if constexpr (MASK == 2) on = on && mk[(int64_t)min(k0 + j, a.Lk - 1) * a.m_sk] != 0;
-          s[hb][r] = on ? s[hb][r] : 0.f;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const Frag f = to_frag<T>(s[hb], i);
-#pragma unroll
-        for (int d = 0; d < DB; ++d) dq[d] = mma(TL::cols(kt, 32 * hb + 16 * i, d, lane), f, dq[d]);
+        const int j = (r >> 2) * 8 + hi * 4 + (r & 3);
+        bool on = k0 + j < lim;
+        if constexpr (MASK == 1) on = on && bs[j] == 0.f;
+        if constexpr (MASK == 2) on = on && mk[(int64_t)min(k0 + j, a.Lk - 1) * a.m_sk] != 0;
+        s[r] = on ? s[r] : 0.f;
       }
     }
+  };
+  auto gradients = [&](const f32x16& s, uint32_t at, int hb) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const Frag f = to_frag<T>(s, i);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) dq[d] = mma(AHEAD ? ck[i][d] : TL::cols(kcol + at, 32 * hb + 16 * i, d), f, dq[d]);
+    }
+  };
+  auto walk = [&](auto edge, int k0, uint32_t at, const float* bs, uint32_t at_next) {
+    if constexpr (NB == 2) {
+      f32x16 s0, p0, s1, p1;
+      products(s0, p0, at, 0);
+      load_rows(at, 1);
+      pin<2 * DT, 1>();
+      products(s1, p1, at, 1);
+      load_cols(at, 0);
+      weights(edge, s0, p0, k0, bs);
+      pin<2 * DT, 1>();
+      gradients(s0, at, 0);
+      load_cols(at, 1);
+      weights(edge, s1, p1, k0 + 32, bs + 32);
+      pin<DT, 2>();
+      gradients(s1, at, 1);
+      load_rows(at_next, 0);
+      pin<DT, 2>();
+    } else {
+      f32x16 s, dp;
+      products(s, dp, at, 0);
+      weights(edge, s, dp, k0, bs);
+      gradients(s, at, 0);
+    }
+  };
+  uint32_t b0 = 0, b1 = 2 * TILE, b2 = 4 * TILE;
+  int s0 = 0, s1 = BK, s2 = 2 * BK;
+  auto turn = [&](auto edge, int t) {
+    raft_wait_vmcnt<0>();
+    __syncthreads();
+    if (t + 2 < t1) issue(t + 2, b2, s2);
+    walk(edge, t * BK, b0, bias + s0, b1);
+    const uint32_t x = b0;
+    b0 = b1, b1 = b2, b2 = x;
+    const int y = s0;
+    s0 = s1, s1 = s2, s2 = y;
+  };
+  if (t0 < t1) {
+    issue(t0, b0, s0);
+    if (t0 + 1 < t1) issue(t0 + 1, b1, s1);
+    raft_wait_vmcnt<0>();
+    __syncthreads();
+    if constexpr (AHEAD) load_rows(b0, 0);
+    int t = t0;
+    if constexpr (MASK == 0)
+      for (const int te = min(t1, bmin / BK); t < te; ++t) turn(Bool<false>{}, t);
+    for (; t < t1; ++t) turn(Bool<true>{}, t);
   }
   if (!ok) return;
   const int64_t o = (((int64_t)b * a.Lq + qi) * a.Hkv * a.G + h) * a.D, n = (int64_t)a.B * a.Lq * a.Hkv * a.G * a.D;
@@ -428,8 +554,8 @@ __device__ __forceinline__ void dq_body(const AttnArgs& a, int bid, int grid, ui
 }
 
 template <typename T, int DP, int MASK>
-__global__ __launch_bounds__(256, 1) void attn_bwd_kernel(AttnArgs a, int grid_kv, int grid_q) {
-  __shared__ __attribute__((aligned(16))) uint8_t sm[4 * BwdCfg<T, DP>::TILE + 4 * BwdCfg<T, DP>::BT * 4];
+__global__ __launch_bounds__(256, (bwd_waves<T, DP>)) __attribute__((amdgpu_waves_per_eu(bwd_waves<T, DP>, bwd_waves<T, DP>))) void attn_bwd_kernel(AttnArgs a, int grid_kv, int grid_q) {
+  __shared__ __attribute__((aligned(16))) uint8_t sm[6 * BwdCfg<T, DP>::TILE + 6 * BwdCfg<T, DP>::BT * 4];
   if ((int)blockIdx.x < grid_kv) dkv_body<T, DP, MASK>(a, blockIdx.x, grid_kv, sm);
   else dq_body<T, DP, MASK>(a, blockIdx.x - grid_kv, grid_q, sm);
 }

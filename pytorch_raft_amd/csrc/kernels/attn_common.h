@@ -77,35 +77,55 @@ struct Tile {
   }
   using Frag = typename FragOf<T>::type;
 
-  // fragment of a row-major tile: elements 16 t + hi * 8 .. + 7 of row `row`
-  __device__ static __forceinline__ Frag rows(const uint8_t* base, int row, int t, int hi) {
-    const uint8_t* p = base + row * RB;
-    const int s = swz(row);
+  // swz is linear over xor and uses row bits 0..3 only, and what depends on the lane and what is known
+  // at compile time never share a bit of row or chunk.  So one register per view of a tile (rows_base,
+  // cols_base: byte addresses in LDS) gives every address by an xor of a constant into the chunk bits
+  // (MASK) and an immediate offset.
+  static constexpr int MASK = RB % 256 == 0 ? 15 : RB % 128 == 0 ? 7 : 3;
+  template <typename V>
+  __device__ static __forceinline__ V at(uint32_t base, int c, int off) {
+    return *reinterpret_cast<const __attribute__((address_space(3))) V*>((base ^ ((uint32_t)(c & MASK) << 4)) + (uint32_t)((c & ~MASK) * 16 + off));
+  }
+
+  // rows view: fragment t of row 32 * rb + (lane & 31) = its elements 16 t + hi * 8 .. + 7
+  __device__ static __forceinline__ uint32_t rows_base(uint32_t lds, int lane) {
+    const int row = lane & 31, hi = lane >> 5;
+    return lds + row * RB + (((ES == 2 ? hi : 2 * hi) ^ swz(row)) << 4);
+  }
+  __device__ static __forceinline__ Frag rows(uint32_t base, int rb, int t) {
     if constexpr (ES == 2) {
-      return *reinterpret_cast<const Frag*>(p + (((2 * t + hi) ^ s) << 4));
+      return at<Frag>(base, 2 * t, rb * 32 * RB);
     } else {
-      const f32x4 a = *reinterpret_cast<const f32x4*>(p + (((4 * t + 2 * hi) ^ s) << 4));
-      const f32x4 b = *reinterpret_cast<const f32x4*>(p + (((4 * t + 2 * hi + 1) ^ s) << 4));
+      const f32x4 a = at<f32x4>(base, 4 * t, rb * 32 * RB);
+      const f32x4 b = at<f32x4>(base, 4 * t + 1, rb * 32 * RB);
       return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
-  // transposed fragment: column 32 * cb + (lane & 31), rows r0 + hi * 4 + {0..3}, r0 + 8 + hi * 4 + {0..3}
-  __device__ static __forceinline__ Frag cols(const uint8_t* base, int r0, int cb, int lane) {
+  // columns view: column 32 * cb + (lane & 31), rows r0 + hi * 4 + {0..3}, r0 + 8 + hi * 4 + {0..3}
+  // (r0 a multiple of 16)
+  __device__ static __forceinline__ uint32_t cols_base(uint32_t lds, int lane) {
     if constexpr (ES == 2) {
-      const int row = r0 + (lane >> 5) * 4 + ((lane & 15) >> 2);
-      const int col = cb * 32 + ((lane >> 4) & 1) * 16 + 4 * (lane & 3);
-      const int o0 = row * RB + (((col >> 3) ^ swz(row)) << 4) + (col & 7) * 2;
-      const int o1 = (row + 8) * RB + (((col >> 3) ^ swz(row + 8)) << 4) + (col & 7) * 2;
-      const v4bf lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4bf*)(base + o0));
-      const v4bf hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4bf*)(base + o1));
+      const int row = (lane >> 5) * 4 + ((lane & 15) >> 2), col = ((lane >> 4) & 1) * 16 + 4 * (lane & 3);
+      return lds + row * RB + (((col >> 3) ^ swz(row)) << 4) + (col & 7) * 2;
+    } else {
+      const int row = (lane >> 5) * 4, col = lane & 31;
+      return lds + row * RB + (((col >> 2) ^ swz(row)) << 4) + (col & 3) * 4;
+    }
+  }
+  __device__ static __forceinline__ Frag cols(uint32_t base, int r0, int cb) {
+    if constexpr (ES == 2) {
+      const int c0 = (4 * cb) ^ swz(0), c1 = (4 * cb) ^ swz(8);
+      const v4bf lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+          (lds_v4bf*)(size_t)((base ^ ((uint32_t)(c0 & MASK) << 4)) + (uint32_t)((c0 & ~MASK) * 16 + r0 * RB)));
+      const v4bf hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+          (lds_v4bf*)(size_t)((base ^ ((uint32_t)(c1 & MASK) << 4)) + (uint32_t)((c1 & ~MASK) * 16 + (r0 + 8) * RB)));
       return __builtin_bit_cast(Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
-      const int col = cb * 32 + (lane & 31);
       Frag f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int row = r0 + (i >> 2) * 8 + (lane >> 5) * 4 + (i & 3);
-        f[i] = *reinterpret_cast<const float*>(base + row * RB + (((col >> 2) ^ swz(row)) << 4) + (col & 3) * 4);
+        const int row = (i >> 2) * 8 + (i & 3);
+        f[i] = at<float>(base, (8 * cb) ^ swz(row), (r0 + row) * RB);
       }
       return f;
     }
@@ -128,6 +148,25 @@ __device__ __forceinline__ rsrc_t rsrc_of(const void* base, uint32_t bytes) {
 // 1-D grids are padded to a multiple of 8: the dispatcher deals consecutive blocks to the 8 XCDs in
 // turn, so logical order xcd * (n / 8) + slot keeps the blocks that share a key head on one XCD's L2.
 __device__ __forceinline__ int xcd_order(int bid, int grid) { return (bid & 7) * (grid >> 3) + (bid >> 3); }
+
+// workgroup -> (tile, split, batch x key head).  Without causal the blocks of a head stay on one XCD;
+// causal tiles differ in length, so they are dealt over all CUs, longest first.
+__device__ __forceinline__ bool place(const AttnArgs& a, int bid, int grid, int tiles, int nsplit, bool last_first, int& tile, int& split, int& bh) {
+  const int heads = a.B * a.Hkv;
+  const int id = a.causal ? bid : xcd_order(bid, grid);
+  if (id >= tiles * nsplit * heads) return false;
+  if (a.causal) {
+    bh = id % heads;
+    split = id / heads % nsplit;
+    tile = id / heads / nsplit;
+  } else {
+    tile = id % tiles;
+    split = id / tiles % nsplit;
+    bh = id / tiles / nsplit;
+  }
+  if (last_first) tile = tiles - 1 - tile;
+  return true;
+}
 
 // One thread's share of the LDS-DMA of ROWS rows (x DP) by NTHR threads: byte offsets from the
 // tile's first row, fixed over the loop (row pitch `pitch` bytes); rows past the descriptor's end

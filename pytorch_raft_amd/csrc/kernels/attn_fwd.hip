@@ -45,20 +45,20 @@ struct RowState {
   }
   // scores of NB blocks of 32 keys
   template <int NB>
-  __device__ __forceinline__ void scores(const uint8_t* kt, f32x16 (&s)[NB], int lane) const {
+  __device__ __forceinline__ void scores(uint32_t kt, f32x16 (&s)[NB]) const {  // kt: rows view
 #pragma unroll
     for (int b = 0; b < NB; ++b) s[b] = zero16();
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
       for (int b = 0; b < NB; ++b)
-        s[b] = mma(TL::rows(kt, b * 32 + (lane & 31), t, lane >> 5), q[t], s[b]);
+        s[b] = mma(TL::rows(kt, b, t), q[t], s[b]);
   }
-  // scores -> probabilities relative to the running reference, which moves (rescaling the output)
-  // only when a row's maximum has outgrown it by 2^8: the result is the same, since sum and
-  // output carry the same factor, and p <= 2^8 is far from every type's limit.
+  // The running reference exponent moves (rescaling sum and output) only when a row's maximum has
+  // outgrown it by 2^8: the result is the same, since both carry the same factor, and p <= 2^8 is far
+  // from every type's limit.
   template <int NB>
-  __device__ __forceinline__ void softmax(f32x16 (&s)[NB], float c) {
+  __device__ __forceinline__ void raise(const f32x16 (&s)[NB], float c) {
     float mx = s[0][0];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -75,6 +75,10 @@ struct RowState {
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[i][r] *= al;
     }
+  }
+  // scores -> probabilities relative to the reference
+  template <int NB>
+  __device__ __forceinline__ void probs(f32x16 (&s)[NB], float c) {
     const float ms = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -85,14 +89,14 @@ struct RowState {
       }
   }
   template <int NB>
-  __device__ __forceinline__ void values(const uint8_t* vt, const f32x16 (&s)[NB], int lane) {
+  __device__ __forceinline__ void values(uint32_t vt, const f32x16 (&s)[NB]) {  // vt: columns view
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const Frag p = to_frag<T>(s[b], t);
 #pragma unroll
-        for (int i = 0; i < DB; ++i) o[i] = mma(TL::cols(vt, b * 32 + 16 * t, i, lane), p, o[i]);
+        for (int i = 0; i < DB; ++i) o[i] = mma(TL::cols(vt, b * 32 + 16 * t, i), p, o[i]);
       }
   }
 };
@@ -134,7 +138,7 @@ __device__ __forceinline__ void store_row(T* p, const f32x16 (&o)[DB], float f, 
 }
 
 template <typename T, int DP, int MASK>
-__global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_fwd_kernel(AttnArgs a) {
   using C = FwdCfg<T, DP>;
   using TL = Tile<T, DP>;
   constexpr int BK = C::BK, NB = BK / 32;
@@ -179,10 +183,13 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
   const uint32_t lds = raft_lds_addr(&kv[0][0][0]) + wave * 1024;
   const uint8_t* mk = MASK ? a.mask + b * a.m_sb + (MASK == 2 ? h * a.m_sh + (int64_t)qi * a.m_sq : 0) : nullptr;
 
-  auto issue = [&](int t, int buf) {
-    const int k0 = t * BK, n = min(BK, len - k0);
-    const rsrc_t rk = rows_rsrc(kb + (int64_t)k0 * kp, n, kp, a.D * TL::ES);
-    const rsrc_t rv = rows_rsrc(vb + (int64_t)k0 * vp, n, vp, a.D * TL::ES);
+  // K runs a tile ahead of V: the scores of tile t + 1 (matrix unit) are formed while tile t goes
+  // through its exponentials (vector unit)
+  auto issue = [&](int t, bool keys) {
+    const int k0 = t * BK, n = min(BK, len - k0), buf = (t - t0) & 1;
+    const uint32_t at = lds + (2 * buf + (keys ? 0 : 1)) * C::TILE;
+    const rsrc_t rs = keys ? rows_rsrc(kb + (int64_t)k0 * kp, n, kp, a.D * TL::ES) : rows_rsrc(vb + (int64_t)k0 * vp, n, vp, a.D * TL::ES);
+    const Loader<T, DP, BK, 256>& ld = keys ? lk : lv;
     if constexpr (MASK == 1) {
       // a hidden key's row is not fetched at all (zeros), whatever it holds
       using L = Loader<T, DP, BK, 256>;
@@ -190,30 +197,29 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
       for (int j = 0; j < L::PER; ++j) {
         const int r = L::row_of(tid, j);
         const bool see = r < n && mk[(int64_t)(k0 + min(r, n - 1)) * a.m_sk] != 0;
-        raft_dma16(rk, lds + (2 * buf) * C::TILE + j * 4096, see ? lk.off[j] : kOob);
-        raft_dma16(rv, lds + (2 * buf + 1) * C::TILE + j * 4096, see ? lv.off[j] : kOob);
+        raft_dma16(rs, at + j * 4096, see ? ld.off[j] : kOob);
       }
-      if (tid < BK) bias[buf][tid] = tid < n && mk[(int64_t)(k0 + min(tid, n - 1)) * a.m_sk] != 0 ? 0.f : -INFINITY;
+      if (keys && tid < BK) bias[buf][tid] = tid < n && mk[(int64_t)(k0 + min(tid, n - 1)) * a.m_sk] != 0 ? 0.f : -INFINITY;
     } else {
-      lk.issue(rk, lds + (2 * buf) * C::TILE);
-      lv.issue(rv, lds + (2 * buf + 1) * C::TILE);
+      ld.issue(rs, at);
     }
   };
-
-  if (t0 < t1) issue(t0, 0);
+  const uint32_t krow = TL::rows_base(raft_lds_addr(&kv[0][0][0]), lane), vcol = TL::cols_base(raft_lds_addr(&kv[0][1][0]), lane);
+  const float c = a.scale_log2;
+  if (t0 < t1) issue(t0, true), issue(t0, false);
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1, k0 = t * BK;
     raft_wait_vmcnt<0>();
     __syncthreads();  // tile t has landed for all waves, and all have left tile t - 1's buffer
-    if (t + 1 < t1) issue(t + 1, buf ^ 1);
-    if (k0 < wlim) {
-      f32x16 s[NB];
-      st.scores(&kv[buf][0][0], s, lane);
-      if (MASK || k0 + BK > wmin)
-        hide<NB, MASK>(s, lim - k0, hi, bias[buf], MASK == 2 ? mk + (int64_t)k0 * a.m_sk : nullptr, a.m_sk, a.Lk - k0);
-      st.softmax(s, a.scale_log2);
-      st.values(&kv[buf][1][0], s, lane);
-    }
+    if (t + 1 < t1) issue(t + 1, true), issue(t + 1, false);
+    if (k0 >= wlim) continue;
+    f32x16 s[NB];
+    st.scores(krow + buf * 2 * C::TILE, s);
+    if (MASK || k0 + BK > wmin)
+      hide<NB, MASK>(s, lim - k0, hi, bias[buf], MASK == 2 ? mk + (int64_t)k0 * a.m_sk : nullptr, a.m_sk, a.Lk - k0);
+    st.raise(s, c);
+    st.probs(s, c);
+    st.values(vcol + buf * 2 * C::TILE, s);
   }
 
   const float l = st.l + other_half(st.l);
@@ -275,8 +281,8 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnArgs a) {
   L lk, lv;
   lk.init(lane, kp, a.D * TL::ES);
   lv.init(lane, vp, a.D * TL::ES);
-  uint8_t* mine = sm + wave * 2 * BUFS * TILE;
   const uint32_t lds = raft_lds_addr(sm) + wave * 2 * BUFS * TILE;
+  const uint32_t krow = TL::rows_base(lds, lane), vcol = TL::cols_base(lds + TILE, lane);
   const uint8_t* mk = MASK ? a.mask + b * a.m_sb + (MASK == 2 ? h * a.m_sh + (int64_t)qi * a.m_sq : 0) : nullptr;
 
   auto issue = [&](int t, int buf) {
@@ -316,7 +322,7 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnArgs a) {
     __builtin_amdgcn_wave_barrier();
     asm volatile("" ::: "memory");
     f32x16 s[1];
-    st.scores(mine + (2 * buf) * TILE, s, lane);
+    st.scores(krow + 2 * buf * TILE, s);
     if (MASK || k0 + 32 > wmin) {
       if constexpr (MASK == 1) {
         const int64_t left = len - 1 - k0;
@@ -330,8 +336,9 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnArgs a) {
         hide<1, MASK>(s, lim - k0, hi, nullptr, MASK == 2 ? mk + (int64_t)k0 * a.m_sk : nullptr, a.m_sk, a.Lk - k0);
       }
     }
-    st.softmax(s, a.scale_log2);
-    st.values(mine + (2 * buf + 1) * TILE, s, lane);
+    st.raise(s, a.scale_log2);
+    st.probs(s, a.scale_log2);
+    st.values(vcol + 2 * buf * TILE, s);
     asm volatile("" ::: "memory");
   }
 
@@ -435,15 +442,14 @@ void fwd_dim(const AttnArgs& a, hipStream_t s) {
 
 }  // namespace attn_detail
 
-int attn_splits(const AttnArgs& a) {
+void attn_fwd_plan(AttnArgs& a) {
+  const int64_t R = (int64_t)a.G * a.Lq, heads = (int64_t)a.B * a.Hkv;
   // Enough workgroups for the 256 CUs: key ranges are split (and joined by a second launch) when the
   // row tiles alone leave CUs idle; a range keeps at least 256 keys so the join stays small.
-  const int64_t R = (int64_t)a.G * a.Lq;
-  const int64_t n = (R <= 32 ? 1 : (R + 127) / 128) * a.B * a.Hkv;
+  const int64_t n = (R <= 32 ? 1 : (R + 127) / 128) * heads;
   const int64_t want = R <= 32 ? 512 : 256;
-  int64_t s = n > 0 ? want / n : 1;
-  s = std::min<int64_t>(s, (a.Lk + 255) / 256);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(s, 64));
+  const int64_t s = std::min<int64_t>(want / std::max<int64_t>(n, 1), (a.Lk + 255) / 256);
+  a.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(s, 64));
 }
 
 void launch_attn_fwd(const AttnArgs& a, hipStream_t s) {

@@ -482,7 +482,7 @@ struct AttnArgs {
   float* part_q;          // (nsplit_q, dq); part holds (2, nsplit_kv, dk) then
   void *dq, *dk, *dv;     // contiguous (B, L, heads, D)
 };
-int attn_splits(const AttnArgs& a);
+void attn_fwd_plan(AttnArgs& a);  // nsplit
 void launch_attn_fwd(const AttnArgs& a, hipStream_t s);
 void attn_bwd_plan(AttnArgs& a);  // nprep, nsplit_kv, nsplit_q
 void launch_attn_bwd(const AttnArgs& a, hipStream_t s);
