@@ -19,6 +19,17 @@ __device__ __forceinline__ rsrc_t rsrc_of(const void* base, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
 }
 
+// pins a run of M matrix instructions with R LDS reads spread between them (M a multiple of R)
+template <int M, int R>
+__device__ __forceinline__ void pin8() {
+  if constexpr (R > 0) {
+    constexpr int K = M / R > 0 ? M / R : 1;
+    __builtin_amdgcn_sched_group_barrier(0x008, K, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    pin8<M - K, R - 1>();
+  }
+}
+
 // 16 bytes of row p at byte k, zeros from K on, any alignment
 __device__ __forceinline__ i32x4 load16(const int8_t* p, int k, int K) {
   i32x4 r = {0, 0, 0, 0};
@@ -55,15 +66,17 @@ __device__ __forceinline__ void store4(const Int8Args& a, int m, int n, i32x4 ac
   }
 }
 
-// ---- tiles: BM tokens x BN channels, BK bytes of k a step, double-buffered LDS filled by LDS-DMA
-// (rows on 16 bytes) or through registers (any K).  A 16-byte chunk c of row r lies in slot
-// c ^ ((r >> 1) & 7): 16 rows of one chunk then cover all banks.
+// ---- tiles: BM tokens x BN channels, BK bytes of k a step, four LDS stages.  Stage t + 1 has landed
+// when step t begins, so a step's last products run beside the reads of the next step's first
+// fragments.  Rows on 16 bytes come by LDS-DMA (two steps in flight), any other through registers
+// (loaded one step, written the next).  A 16-byte chunk c of row r lies in slot c ^ ((r >> 2) & 3):
+// 16 rows of one chunk then cover all banks.
 template <int BM, int BN, int WVM, bool ALIGNED, typename T>
 __global__ __launch_bounds__(256, (BM * BN <= 128 * 128 ? 2 : 1)) void int8_tile_kernel(Int8Args a) {
-  constexpr int BK = 128, WVN = 4 / WVM, WM = BM / WVM, WN = BN / WVN, TM = WM / 32, TN = WN / 32;
+  constexpr int BK = 64, NS = 4, WVN = 4 / WVM, WM = BM / WVM, WN = BN / WVN, TM = WM / 32, TN = WN / 32;
   constexpr int STAGE = (BM + BN) * BK;
-  constexpr int PER = (BM + BN) * 8 / 256;
-  __shared__ __attribute__((aligned(16))) uint8_t sm[2][STAGE];
+  constexpr int PER = (BM + BN) * 4 / 256;
+  __shared__ __attribute__((aligned(16))) uint8_t sm[NS][STAGE];
 
   const int mt = (a.M + BM - 1) / BM, nt = (a.N + BN - 1) / BN;
   const int id = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
@@ -82,25 +95,58 @@ __global__ __launch_bounds__(256, (BM * BN <= 128 * 128 ? 2 : 1)) void int8_tile
   const rsrc_t rx = rsrc_of(x, (uint32_t)mrows * (uint32_t)a.K), rw = rsrc_of(w, (uint32_t)nrows * (uint32_t)a.K);
   const uint32_t lds = raft_lds_addr(&sm[0][0]) + wave * 1024;
 
-  // x rows first, then w rows
-  auto issue = [&](int k0, int buf) {
+  // this thread's chunks: x rows first, then w rows (rows past the last read as zeros)
+  uint32_t off[PER];
+  int kc[PER];
+  bool ok[PER];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int e = j * 256 + tid, row = e >> 3, c = (e & 7) ^ ((row >> 1) & 7), k = k0 + c * 16;
-      const bool isx = j * 256 < BM * 8;
-      const int r = isx ? row : row - BM;
-      if constexpr (ALIGNED) {
-        const bool ok = k < a.K && r < (isx ? mrows : nrows);
-        raft_dma16(isx ? rx : rw, lds + buf * STAGE + j * 4096, ok ? (uint32_t)r * (uint32_t)a.K + k : kOob);
-      } else {
-        i32x4 v = {0, 0, 0, 0};
-        if (r < (isx ? mrows : nrows)) v = load16((isx ? x : w) + (int64_t)r * a.K, k, a.K);
-        *reinterpret_cast<i32x4*>(&sm[buf][e * 16]) = v;
-      }
+  for (int j = 0; j < PER; ++j) {
+    const int e = j * 256 + tid, row = e >> 2, c = (e & 3) ^ ((row >> 2) & 3);
+    const bool isx = j * 256 < BM * 4;
+    const int r = isx ? row : row - BM;
+    ok[j] = r < (isx ? mrows : nrows);
+    kc[j] = c * 16;
+    off[j] = ok[j] ? (uint32_t)r * (uint32_t)a.K + c * 16 : kOob;
+  }
+  auto issue = [&](int t) {
+    const uint32_t at = lds + (t & (NS - 1)) * STAGE;
+    const int k0 = t * BK;
+    if (k0 + BK <= a.K) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) raft_dma16(j * 256 < BM * 4 ? rx : rw, at + j * 4096, off[j] + k0);
+    } else {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) raft_dma16(j * 256 < BM * 4 ? rx : rw, at + j * 4096, k0 + kc[j] < a.K ? off[j] + k0 : kOob);
     }
   };
-  auto frag = [&](const uint8_t* base, int row, int kk) {
-    return *reinterpret_cast<const i32x4*>(base + row * BK + (((2 * kk + hi) ^ ((row >> 1) & 7)) << 4));
+  i32x4 hold[ALIGNED ? 1 : PER];
+  auto fetch = [&](int t) {
+    const int k0 = t * BK;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int8_t* p = (j * 256 < BM * 4 ? x : w) + (ok[j] ? off[j] : 0);
+      if (k0 + BK <= a.K) __builtin_memcpy(&hold[j], p + k0, 16);
+      else hold[j] = load16(p - kc[j] * (ok[j] ? 1 : 0), k0 + kc[j], a.K);
+      if (!ok[j]) hold[j] = i32x4{0, 0, 0, 0};
+    }
+  };
+  auto put = [&](int t) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) *reinterpret_cast<i32x4*>(&sm[t & (NS - 1)][(j * 256 + tid) * 16]) = hold[j];
+  };
+
+  // fragment addresses: row * 64 + ((2 kk + hi) ^ swizzle) * 16, kk by an xor of 32
+  const int sw = (lane >> 2) & 3;
+  const uint32_t fbase = raft_lds_addr(&sm[0][0]) + (lane & 31) * BK + ((hi ^ sw) << 4);
+  const uint32_t xbase = fbase + wm * BK, wbase = fbase + (BM + wn) * BK;
+  i32x4 fx[2][TM], fw[2][TN];
+  auto frags = [&](int s, int t, int kk) {
+    const uint32_t at = (t & (NS - 1)) * STAGE;
+    const uint32_t px = (xbase ^ (kk * 32)) + at, pw = (wbase ^ (kk * 32)) + at;
+#pragma unroll
+    for (int j = 0; j < TM; ++j) fx[s][j] = *reinterpret_cast<const __attribute__((address_space(3))) i32x4*>(px + 32 * j * BK);
+#pragma unroll
+    for (int i = 0; i < TN; ++i) fw[s][i] = *reinterpret_cast<const __attribute__((address_space(3))) i32x4*>(pw + 32 * i * BK);
   };
 
   i32x16 acc[TN][TM];
@@ -110,41 +156,99 @@ __global__ __launch_bounds__(256, (BM * BN <= 128 * 128 ? 2 : 1)) void int8_tile
     for (int j = 0; j < TM; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
+  auto products = [&](int s) {
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+      for (int j = 0; j < TM; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[s][i], fx[s][j], acc[i][j], 0, 0, 0);
+  };
 
   const int steps = (a.K + BK - 1) / BK;
-  issue(0, 0);
-  for (int t = 0; t < steps; ++t) {
-    const int buf = t & 1;
-    raft_wait_vmcnt<0>();
-    __syncthreads();
-    if (t + 1 < steps) issue((t + 1) * BK, buf ^ 1);
-    const uint8_t* xt = &sm[buf][0];
-    const uint8_t* wt = &sm[buf][BM * BK];
-#pragma unroll
-    for (int kk = 0; kk < BK / 32; ++kk) {
-      i32x4 fx[TM], fw[TN];
-#pragma unroll
-      for (int j = 0; j < TM; ++j) fx[j] = frag(xt, wm + 32 * j + (lane & 31), kk);
-#pragma unroll
-      for (int i = 0; i < TN; ++i) fw[i] = frag(wt, wn + 32 * i + (lane & 31), kk);
-#pragma unroll
-      for (int i = 0; i < TN; ++i)
-#pragma unroll
-        for (int j = 0; j < TM; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[i], fx[j], acc[i][j], 0, 0, 0);
+  if (steps > 0) {
+    if constexpr (ALIGNED) {
+      issue(0);
+      if (1 < steps) issue(1);
+      if (2 < steps) issue(2);
+      if (2 < steps) raft_wait_vmcnt<2 * PER>();
+      else raft_wait_vmcnt<0>();
+    } else {
+      fetch(0);
+      put(0);
+      if (1 < steps) fetch(1), put(1);
+      if (2 < steps) fetch(2);
     }
+    __syncthreads();
+    frags(0, 0, 0);
   }
+  for (int t = 0; t < steps; ++t) {
+    if constexpr (ALIGNED) {
+      if (t + 2 < steps) raft_wait_vmcnt<PER>();
+      else raft_wait_vmcnt<0>();
+    }
+    __syncthreads();  // stage t + 1 has landed for all waves, and all have left stage t - 1
+    if constexpr (ALIGNED) {
+      if (t + 3 < steps) issue(t + 3);
+    } else {
+      if (t + 2 < steps) put(t + 2);
+      if (t + 3 < steps) fetch(t + 3);
+    }
+    products(0);
+    frags(1, t, 1);
+    pin8<TM * TN, TM + TN>();
+    products(1);
+    frags(0, t + 1, 0);  // (past the last step: a stage that was read before, unused)
+    pin8<TM * TN, TM + TN>();
+  }
+  // Results go out through LDS, 32 tokens of a wave at a time: a lane holds 4 channels of one token
+  // (stores of 8 bytes in 32 rows took 146 us of the 401 us of 8192 x 8192 x 4096), a row of the buffer
+  // is WN channels in a row.
+  constexpr int ROW = WN * (int)sizeof(T) + 16, CH = 16 / (int)sizeof(T), LPR = WN / CH;  // bytes, channels a chunk, lanes a row
+  static_assert(4 * 32 * ROW + 2 * BN * 4 <= NS * STAGE, "epilogue buffers");
+  __syncthreads();
+  float* scales = reinterpret_cast<float*>(&sm[0][0]);
+  uint8_t* buf = &sm[0][0] + 2 * BN * 4 + wave * 32 * ROW;
+  for (int i = tid; i < BN; i += 256) {
+    scales[i] = n0 + i < a.N ? a.ws[n0 + i] : 0.f;
+    scales[BN + i] = a.bias && n0 + i < a.N ? a.bias[n0 + i] : 0.f;
+  }
+  __syncthreads();
 #pragma unroll
   for (int j = 0; j < TM; ++j) {
-    const int m = m0 + wm + 32 * j + (lane & 31);
-    if (m >= a.M) continue;
-    const float xs = a.xs[m];
+    const int mb = m0 + wm + 32 * j;
+    const float xs = a.xs[min(mb + (lane & 31), a.M - 1)];
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int n = n0 + wn + 32 * i + 8 * g + 4 * hi;
-        if (n < a.N) store4<T>(a, m, n, i32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]}, xs);
+        const int c = 32 * i + 8 * g + 4 * hi;
+        const f32x4 ws = *reinterpret_cast<const f32x4*>(scales + wn + c), bi = *reinterpret_cast<const f32x4*>(scales + BN + wn + c);
+        typedef T v4 __attribute__((ext_vector_type(4)));
+        v4 r;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r[k] = (T)fmaf((float)acc[i][j][4 * g + k] * xs, ws[k], bi[k]);
+        *reinterpret_cast<v4*>(buf + (lane & 31) * ROW + c * (int)sizeof(T)) = r;
       }
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int q = 0; q < 32 * LPR / 64; ++q) {
+      const int row = (q * 64 + lane) / LPR, c = (lane % LPR) * CH, m = mb + row, n = n0 + wn + c;
+      const uint4 v = *reinterpret_cast<const uint4*>(buf + row * ROW + c * (int)sizeof(T));
+      T* o = reinterpret_cast<T*>(a.out) + (int64_t)m * a.N + n;
+      if (m < a.M) {
+        if (n + CH <= a.N) {
+          __builtin_memcpy(o, &v, 16);
+        } else {
+          T e[CH];
+          __builtin_memcpy(e, &v, 16);
+#pragma unroll
+          for (int k = 0; k < CH; ++k)
+            if (n + k < a.N) o[k] = e[k];
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
   }
 }
 
