@@ -290,6 +290,11 @@ Tensor int8_mm(const Tensor& x, const Tensor& xs, const Tensor& w, const Tensor&
   a.N = (int)N;
   a.K = (int)K;
   a.dtype = (int)out_dtype;
+  Tensor packed;
+  if (const int64_t n = int8_packed_bytes(a)) {
+    packed = at::empty({n}, x.options());
+    a.packed = packed.data_ptr<int8_t>();
+  }
   launch_int8_mm(a, cur_stream());
   return out;
 }

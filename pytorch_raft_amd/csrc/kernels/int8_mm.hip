@@ -13,28 +13,24 @@ namespace int8_detail {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
+template <bool V>
+struct Bool {
+  static constexpr bool value = V;
+};
 constexpr uint32_t kOob = 0x80000000u;
 
 __device__ __forceinline__ rsrc_t rsrc_of(const void* base, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
 }
 
-// pins a run of M matrix instructions with R LDS reads spread between them (M a multiple of R)
-template <int M, int R>
-__device__ __forceinline__ void pin8() {
-  if constexpr (R > 0) {
-    constexpr int K = M / R > 0 ? M / R : 1;
-    __builtin_amdgcn_sched_group_barrier(0x008, K, 0);
-    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-    pin8<M - K, R - 1>();
-  }
-}
-
-// 16 bytes of row p at byte k, zeros from K on, any alignment
+// 16 bytes of row p at byte k, zeros from K on, any alignment.  The last piece of a row is the row's
+// last 16 bytes, shifted.
 __device__ __forceinline__ i32x4 load16(const int8_t* p, int k, int K) {
   i32x4 r = {0, 0, 0, 0};
-  if (k + 16 <= K) {
-    __builtin_memcpy(&r, p + k, 16);
+  if (K >= 16) {
+    if (k < K) __builtin_memcpy(&r, p + min(k, K - 16), 16);
+    const int drop = max(0, min(k, K) + 16 - K);
+    if (drop > 0) r = __builtin_bit_cast(i32x4, drop < 16 ? __builtin_bit_cast(unsigned __int128, r) >> (8 * drop) : (unsigned __int128)0);
   } else if (k < K) {
 #pragma unroll
     for (int i = 0; i < 16; ++i)
@@ -108,16 +104,14 @@ __global__ __launch_bounds__(256, (BM * BN <= 128 * 128 ? 2 : 1)) void int8_tile
     kc[j] = c * 16;
     off[j] = ok[j] ? (uint32_t)r * (uint32_t)a.K + c * 16 : kOob;
   }
-  auto issue = [&](int t) {
-    const uint32_t at = lds + (t & (NS - 1)) * STAGE;
+  auto issue = [&](int t, int j) {  // chunk j of stage t (past the last step: zeros that nobody reads)
+    const uint32_t at = lds + (t & (NS - 1)) * STAGE + j * 4096;
     const int k0 = t * BK;
-    if (k0 + BK <= a.K) {
+    raft_dma16(j * 256 < BM * 4 ? rx : rw, at, k0 + kc[j] < a.K ? off[j] + k0 : kOob);
+  };
+  auto issue_all = [&](int t) {
 #pragma unroll
-      for (int j = 0; j < PER; ++j) raft_dma16(j * 256 < BM * 4 ? rx : rw, at + j * 4096, off[j] + k0);
-    } else {
-#pragma unroll
-      for (int j = 0; j < PER; ++j) raft_dma16(j * 256 < BM * 4 ? rx : rw, at + j * 4096, k0 + kc[j] < a.K ? off[j] + k0 : kOob);
-    }
+    for (int j = 0; j < PER; ++j) issue(t, j);
   };
   i32x4 hold[ALIGNED ? 1 : PER];
   auto fetch = [&](int t) {
@@ -140,13 +134,11 @@ __global__ __launch_bounds__(256, (BM * BN <= 128 * 128 ? 2 : 1)) void int8_tile
   const uint32_t fbase = raft_lds_addr(&sm[0][0]) + (lane & 31) * BK + ((hi ^ sw) << 4);
   const uint32_t xbase = fbase + wm * BK, wbase = fbase + (BM + wn) * BK;
   i32x4 fx[2][TM], fw[2][TN];
-  auto frags = [&](int s, int t, int kk) {
+  auto frag = [&](int s, int t, int kk, int f) {  // fragment f: TM of x, then TN of w
     const uint32_t at = (t & (NS - 1)) * STAGE;
-    const uint32_t px = (xbase ^ (kk * 32)) + at, pw = (wbase ^ (kk * 32)) + at;
-#pragma unroll
-    for (int j = 0; j < TM; ++j) fx[s][j] = *reinterpret_cast<const __attribute__((address_space(3))) i32x4*>(px + 32 * j * BK);
-#pragma unroll
-    for (int i = 0; i < TN; ++i) fw[s][i] = *reinterpret_cast<const __attribute__((address_space(3))) i32x4*>(pw + 32 * i * BK);
+    typedef const __attribute__((address_space(3))) i32x4* lds_ptr;
+    if (f < TM) fx[s][f] = *reinterpret_cast<lds_ptr>((xbase ^ (kk * 32)) + at + 32 * f * BK);
+    else fw[s][f - TM] = *reinterpret_cast<lds_ptr>((wbase ^ (kk * 32)) + at + 32 * (f - TM) * BK);
   };
 
   i32x16 acc[TN][TM];
@@ -156,21 +148,30 @@ __global__ __launch_bounds__(256, (BM * BN <= 128 * 128 ? 2 : 1)) void int8_tile
     for (int j = 0; j < TM; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
-  auto products = [&](int s) {
+  // Half a step: the products of fragment set s with, spread between them, the reads of the other set
+  // (stage tf, half kk) and, in the first half, the DMA of stage td.  A DMA in one piece at the top of the
+  // step kept the matrix unit waiting (one wave per SIMD): 292 us at 8192 x 8192 x 4096, 283 spread.
+  auto half = [&](auto dma, int s, int tf, int kk, int td) {
 #pragma unroll
-    for (int i = 0; i < TN; ++i)
+    for (int q = 0; q < TM * TN; ++q) {
+      acc[q / TM][q % TM] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[s][q / TM], fx[s][q % TM], acc[q / TM][q % TM], 0, 0, 0);
 #pragma unroll
-      for (int j = 0; j < TM; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[s][i], fx[s][j], acc[i][j], 0, 0, 0);
+      for (int f = q * (TM + TN) / (TM * TN); f < (q + 1) * (TM + TN) / (TM * TN); ++f) frag(s ^ 1, tf, kk, f);
+      if constexpr (ALIGNED && decltype(dma)::value) {
+#pragma unroll
+        for (int j = q * PER / (TM * TN); j < (q + 1) * PER / (TM * TN); ++j) issue(td, j);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
 
   const int steps = (a.K + BK - 1) / BK;
   if (steps > 0) {
     if constexpr (ALIGNED) {
-      issue(0);
-      if (1 < steps) issue(1);
-      if (2 < steps) issue(2);
-      if (2 < steps) raft_wait_vmcnt<2 * PER>();
-      else raft_wait_vmcnt<0>();
+      issue_all(0);
+      issue_all(1);
+      issue_all(2);
+      raft_wait_vmcnt<2 * PER>();
     } else {
       fetch(0);
       put(0);
@@ -178,32 +179,25 @@ __global__ __launch_bounds__(256, (BM * BN <= 128 * 128 ? 2 : 1)) void int8_tile
       if (2 < steps) fetch(2);
     }
     __syncthreads();
-    frags(0, 0, 0);
+#pragma unroll
+    for (int f = 0; f < TM + TN; ++f) frag(0, 0, 0, f);
   }
   for (int t = 0; t < steps; ++t) {
-    if constexpr (ALIGNED) {
-      if (t + 2 < steps) raft_wait_vmcnt<PER>();
-      else raft_wait_vmcnt<0>();
-    }
+    if constexpr (ALIGNED) raft_wait_vmcnt<PER>();
     __syncthreads();  // stage t + 1 has landed for all waves, and all have left stage t - 1
-    if constexpr (ALIGNED) {
-      if (t + 3 < steps) issue(t + 3);
-    } else {
+    if constexpr (!ALIGNED) {
       if (t + 2 < steps) put(t + 2);
       if (t + 3 < steps) fetch(t + 3);
     }
-    products(0);
-    frags(1, t, 1);
-    pin8<TM * TN, TM + TN>();
-    products(1);
-    frags(0, t + 1, 0);  // (past the last step: a stage that was read before, unused)
-    pin8<TM * TN, TM + TN>();
+    half(Bool<true>{}, 0, t, 1, t + 3);
+    half(Bool<false>{}, 1, t + 1, 0, 0);  // (past the last step: whatever the stage holds, unused)
   }
   // Results go out through LDS, 32 tokens of a wave at a time: a lane holds 4 channels of one token
   // (stores of 8 bytes in 32 rows took 146 us of the 401 us of 8192 x 8192 x 4096), a row of the buffer
   // is WN channels in a row.
   constexpr int ROW = WN * (int)sizeof(T) + 16, CH = 16 / (int)sizeof(T), LPR = WN / CH;  // bytes, channels a chunk, lanes a row
   static_assert(4 * 32 * ROW + 2 * BN * 4 <= NS * STAGE, "epilogue buffers");
+  raft_wait_vmcnt<0>();  // (the stages past the last)
   __syncthreads();
   float* scales = reinterpret_cast<float*>(&sm[0][0]);
   uint8_t* buf = &sm[0][0] + 2 * BN * 4 + wave * 32 * ROW;
@@ -292,11 +286,23 @@ __global__ __launch_bounds__(512) void int8_few_kernel(Int8Args a) {
   }
 }
 
+// x and w with rows of kp (a multiple of 16) bytes, zeros from K on, in `to` (16 bytes a thread)
+__global__ __launch_bounds__(256) void int8_pack_kernel(const int8_t* x, const int8_t* w, int8_t* to, int64_t M, int64_t N, int K, int kp) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = i / (kp / 16);
+  const int k = (int)(i - row * (kp / 16)) * 16;
+  if (row >= M + N) return;
+  const i32x4 v = load16(row < M ? x + row * K : w + (row - M) * K, k, K);
+  *reinterpret_cast<i32x4*>(to + row * kp + k) = v;
+}
+
+bool on16(const Int8Args& a) { return a.K % 16 == 0 && (((uintptr_t)a.x | (uintptr_t)a.w) & 15) == 0; }
+bool whole_tiles(const Int8Args& a) { return a.M > 64 && (int64_t)raft_cdiv(a.M, 256) * raft_cdiv(a.N, 256) >= 256; }
+
 template <int BM, int BN, int WVM, typename T>
 void tile_launch(const Int8Args& a, hipStream_t s) {
   const unsigned grid = raft_cdiv((int64_t)raft_cdiv(a.M, BM) * raft_cdiv(a.N, BN), 8) * 8;
-  const bool aligned = a.K % 16 == 0 && (((uintptr_t)a.x | (uintptr_t)a.w) & 15) == 0;
-  if (aligned) int8_tile_kernel<BM, BN, WVM, true, T><<<grid, 256, 0, s>>>(a);
+  if (on16(a)) int8_tile_kernel<BM, BN, WVM, true, T><<<grid, 256, 0, s>>>(a);
   else int8_tile_kernel<BM, BN, WVM, false, T><<<grid, 256, 0, s>>>(a);
 }
 
@@ -310,13 +316,30 @@ void mm(const Int8Args& a, hipStream_t s) {
     return;
   }
   // the largest tile that still gives every CU one
-  if ((int64_t)raft_cdiv(a.M, 256) * raft_cdiv(a.N, 256) >= 256) tile_launch<256, 256, 2, T>(a, s);
-  else if ((int64_t)raft_cdiv(a.M, 128) * raft_cdiv(a.N, 128) >= 256) tile_launch<128, 128, 2, T>(a, s);
-  else tile_launch<64, 64, 2, T>(a, s);
+  if (whole_tiles(a)) {
+    Int8Args p = a;
+    if (a.packed) {
+      p.K = (a.K + 15) / 16 * 16;
+      p.x = a.packed;
+      p.w = a.packed + (int64_t)a.M * p.K;
+      int8_pack_kernel<<<raft_cdiv(((int64_t)a.M + a.N) * (p.K / 16), 256), 256, 0, s>>>(a.x, a.w, a.packed, a.M, a.N, a.K, p.K);
+    }
+    int8_tile_kernel<256, 256, 2, true, T><<<raft_cdiv((int64_t)raft_cdiv(a.M, 256) * raft_cdiv(a.N, 256), 8) * 8, 256, 0, s>>>(p);
+  } else if ((int64_t)raft_cdiv(a.M, 128) * raft_cdiv(a.N, 128) >= 256) {
+    tile_launch<128, 128, 2, T>(a, s);
+  } else {
+    tile_launch<64, 64, 2, T>(a, s);
+  }
 }
 
 }  // namespace int8_detail
 
+int64_t int8_packed_bytes(const Int8Args& a) {
+  // Products of 256 x 256 tiles read every operand row many times: one copy with rows on 16 bytes
+  // costs less than loads through registers (8192 x 8192 x 4099: 333 us against 538).
+  if (int8_detail::on16(a) || !int8_detail::whole_tiles(a)) return 0;
+  return ((int64_t)a.M + a.N) * ((a.K + 15) / 16 * 16);
+}
 void launch_int8_mm(const Int8Args& a, hipStream_t s) {
   if (a.dtype == 0) int8_detail::mm<__bf16>(a, s);
   else if (a.dtype == 1) int8_detail::mm<_Float16>(a, s);

@@ -511,7 +511,9 @@ void launch_rms_bwd(const RmsArgs& a, hipStream_t s);
 struct Int8Args {
   const int8_t *x, *w;
   const float *xs, *ws, *bias;  // bias nullable
+  int8_t* packed;               // workspace of int8_packed_bytes (null if 0)
   void* out;
   int M, N, K, dtype;
 };
+int64_t int8_packed_bytes(const Int8Args& a);
 void launch_int8_mm(const Int8Args& a, hipStream_t s);
