@@ -379,7 +379,6 @@ __device__ __forceinline__ void dq_body(const AttnArgs& a, int bid, int grid, ui
   constexpr int BK = BwdCfg<T, DP>::BT, TILE = BwdCfg<T, DP>::TILE, DB = DP / 32, DT = DP / 16, NB = BK / 32;
   constexpr bool AHEAD = sizeof(T) == 2;
   constexpr bool F16 = is_f16<T>;
-  float* bias = reinterpret_cast<float*>(sm + 6 * TILE);  // [buffer][key of the tile]
 
   const int R = a.G * a.Lq;
   int tile, split, bh;
@@ -434,23 +433,25 @@ __device__ __forceinline__ void dq_body(const AttnArgs& a, int bid, int grid, ui
   const uint32_t krow = TL::rows_base(raft_lds_addr(sm), lane), kcol = TL::cols_base(raft_lds_addr(sm), lane);
   const uint8_t* mk = MASK ? a.mask + b * a.m_sb + (MASK == 2 ? h * a.m_sh + (int64_t)qi * a.m_sq : 0) : nullptr;
 
-  auto issue = [&](int t, uint32_t buf, int sbuf) {
+  uint8_t byte = 0;  // key mask: the next tile's bytes, and the seen keys of three tiles as bits
+  uint64_t m0 = 0, m1 = 0, m2 = 0;
+  auto look = [&](int t) {
+    if constexpr (MASK == 1) byte = (lane & (BK - 1)) < len - t * BK ? mk[(int64_t)(t * BK + (lane & (BK - 1))) * a.m_sk] : 0;
+  };
+  auto issue = [&](int t, uint32_t buf) {
     const int k0 = t * BK, n = min(BK, len - k0);
     const rsrc_t rk = rows_rsrc(kb + (int64_t)k0 * kp, n, kp, a.D * TL::ES);
     const rsrc_t rv = rows_rsrc(vb + (int64_t)k0 * vp, n, vp, a.D * TL::ES);
+    uint64_t m = 0;
+    if constexpr (MASK == 1) m = __ballot(byte != 0);
 #pragma unroll
     for (int j = 0; j < L::PER; ++j) {
-      bool see = true;
-      if constexpr (MASK == 1) {
-        const int r = L::row_of(tid, j);
-        see = r < n && mk[(int64_t)(k0 + min(r, n - 1)) * a.m_sk] != 0;
-      }
+      const bool see = MASK != 1 || (m >> L::row_of(tid, j) & 1);
       raft_dma16(rk, lds + buf + j * 4096, see ? lk.off[j] : kOob);
       raft_dma16(rv, lds + buf + TILE + j * 4096, see ? lv.off[j] : kOob);
     }
-    if constexpr (MASK == 1) {
-      if (tid < BK) bias[sbuf + tid] = tid < n && mk[(int64_t)(k0 + min(tid, n - 1)) * a.m_sk] != 0 ? 0.f : -INFINITY;
-    }
+    if (t + 1 < t1) look(t + 1);
+    return m;
   };
 
   // (the dk / dv kind's pattern with keys and rows exchanged)
@@ -476,7 +477,7 @@ __device__ __forceinline__ void dq_body(const AttnArgs& a, int bid, int grid, ui
       dp = mma(AHEAD ? fv[i] : TL::rows(krow + at + TILE, hb, i), df[i], dp);
     }
   };
-  auto weights = [&](auto edge, f32x16& s, const f32x16& dp, int k0, const float* bs) {
+  auto weights = [&](auto edge, f32x16& s, const f32x16& dp, int k0, uint32_t keys) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale_log2, sub));
@@ -487,7 +488,7 @@ __device__ __forceinline__ void dq_body(const AttnArgs& a, int bid, int grid, ui
       for (int r = 0; r < 16; ++r) {
         const int j = (r >> 2) * 8 + hi * 4 + (r & 3);
         bool on = k0 + j < lim;
-        if constexpr (MASK == 1) on = on && bs[j] == 0.f;
+        if constexpr (MASK == 1) on = on && (keys >> j & 1);
         if constexpr (MASK == 2) on = on && mk[(int64_t)min(k0 + j, a.Lk - 1) * a.m_sk] != 0;
         s[r] = on ? s[r] : 0.f;
       }
@@ -501,7 +502,7 @@ __device__ __forceinline__ void dq_body(const AttnArgs& a, int bid, int grid, ui
       for (int d = 0; d < DB; ++d) dq[d] = mma(AHEAD ? ck[i][d] : TL::cols(kcol + at, 32 * hb + 16 * i, d), f, dq[d]);
     }
   };
-  auto walk = [&](auto edge, int k0, uint32_t at, const float* bs, uint32_t at_next) {
+  auto walk = [&](auto edge, int k0, uint32_t at, uint64_t keys, uint32_t at_next) {
     if constexpr (NB == 2) {
       f32x16 s0, p0, s1, p1;
       products(s0, p0, at, 0);
@@ -509,11 +510,11 @@ __device__ __forceinline__ void dq_body(const AttnArgs& a, int bid, int grid, ui
       pin<2 * DT, 1>();
       products(s1, p1, at, 1);
       load_cols(at, 0);
-      weights(edge, s0, p0, k0, bs);
+      weights(edge, s0, p0, k0, (uint32_t)keys);
       pin<2 * DT, 1>();
       gradients(s0, at, 0);
       load_cols(at, 1);
-      weights(edge, s1, p1, k0 + 32, bs + 32);
+      weights(edge, s1, p1, k0 + 32, (uint32_t)(keys >> 32));
       pin<DT, 2>();
       gradients(s1, at, 1);
       load_rows(at_next, 0);
@@ -521,25 +522,24 @@ __device__ __forceinline__ void dq_body(const AttnArgs& a, int bid, int grid, ui
     } else {
       f32x16 s, dp;
       products(s, dp, at, 0);
-      weights(edge, s, dp, k0, bs);
+      weights(edge, s, dp, k0, (uint32_t)keys);
       gradients(s, at, 0);
     }
   };
   uint32_t b0 = 0, b1 = 2 * TILE, b2 = 4 * TILE;
-  int s0 = 0, s1 = BK, s2 = 2 * BK;
   auto turn = [&](auto edge, int t) {
     raft_wait_vmcnt<0>();
     __syncthreads();
-    if (t + 2 < t1) issue(t + 2, b2, s2);
-    walk(edge, t * BK, b0, bias + s0, b1);
+    if (t + 2 < t1) m2 = issue(t + 2, b2);
+    walk(edge, t * BK, b0, m0, b1);
     const uint32_t x = b0;
     b0 = b1, b1 = b2, b2 = x;
-    const int y = s0;
-    s0 = s1, s1 = s2, s2 = y;
+    m0 = m1, m1 = m2;
   };
   if (t0 < t1) {
-    issue(t0, b0, s0);
-    if (t0 + 1 < t1) issue(t0 + 1, b1, s1);
+    look(t0);
+    m0 = issue(t0, b0);
+    if (t0 + 1 < t1) m1 = issue(t0 + 1, b1);
     raft_wait_vmcnt<0>();
     __syncthreads();
     if constexpr (AHEAD) load_rows(b0, 0);

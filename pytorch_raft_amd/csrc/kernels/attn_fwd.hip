@@ -101,22 +101,22 @@ struct RowState {
   }
 };
 
-// keys at or past `lim` (this lane's row) and keys hidden by the mask -> -inf.  bias: per-key 0 / -inf
-// of a key mask (LDS); full: this row's bytes of a (query, key) mask at the tile's first key.
+// keys from `left` on (this lane's row) and keys hidden by the mask -> -inf.  keys: bits of the tile's
+// seen keys (key mask); full: this row's bytes of a (query, key) mask at the tile's first key.
 template <int NB, int MASK>
-__device__ __forceinline__ void hide(f32x16 (&s)[NB], int left, int hi, const float* bias, const uint8_t* full,
-                                     int64_t msk, int nkeys) {
+__device__ __forceinline__ void hide(f32x16 (&s)[NB], int left, int hi, uint64_t keys, const uint8_t* full, int64_t msk, int nkeys) {
 #pragma unroll
-  for (int b = 0; b < NB; ++b)
+  for (int b = 0; b < NB; ++b) {
+    const uint32_t bits = (uint32_t)(keys >> (32 * b)) >> (4 * hi);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int j = b * 32 + (r >> 2) * 8 + hi * 4 + (r & 3);
-      float v = s[b][r];
-      if constexpr (MASK == 1) v += bias[j];
       bool see = j < left;
+      if constexpr (MASK == 1) see = see && (bits >> ((r >> 2) * 8 + (r & 3)) & 1);
       if constexpr (MASK == 2) see = see && j < nkeys && full[min(j, nkeys - 1) * msk] != 0;
-      s[b][r] = see ? v : -INFINITY;
+      s[b][r] = see ? s[b][r] : -INFINITY;
     }
+  }
 }
 
 // lane's output row (column of O^T): 4 consecutive channels per 4 registers
@@ -143,7 +143,6 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
   using TL = Tile<T, DP>;
   constexpr int BK = C::BK, NB = BK / 32;
   __shared__ __attribute__((aligned(16))) uint8_t kv[2][2][C::TILE];
-  __shared__ __attribute__((aligned(16))) float bias[2][BK];
 
   const int R = a.G * a.Lq;
   const int tiles = (R + C::BM - 1) / C::BM;
@@ -183,40 +182,46 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
   const uint32_t lds = raft_lds_addr(&kv[0][0][0]) + wave * 1024;
   const uint8_t* mk = MASK ? a.mask + b * a.m_sb + (MASK == 2 ? h * a.m_sh + (int64_t)qi * a.m_sq : 0) : nullptr;
 
-  // K runs a tile ahead of V: the scores of tile t + 1 (matrix unit) are formed while tile t goes
-  // through its exponentials (vector unit)
-  auto issue = [&](int t, bool keys) {
-    const int k0 = t * BK, n = min(BK, len - k0), buf = (t - t0) & 1;
-    const uint32_t at = lds + (2 * buf + (keys ? 0 : 1)) * C::TILE;
-    const rsrc_t rs = keys ? rows_rsrc(kb + (int64_t)k0 * kp, n, kp, a.D * TL::ES) : rows_rsrc(vb + (int64_t)k0 * vp, n, vp, a.D * TL::ES);
-    const Loader<T, DP, BK, 256>& ld = keys ? lk : lv;
-    if constexpr (MASK == 1) {
-      // a hidden key's row is not fetched at all (zeros), whatever it holds
-      using L = Loader<T, DP, BK, 256>;
+  // key mask: each wave looks a tile ahead at the tile's bytes and keeps them as bits
+  uint8_t byte = 0;
+  uint64_t keys = 0;
+  auto look = [&](int t) {
+    if constexpr (MASK == 1) byte = (lane & (BK - 1)) < len - t * BK ? mk[(int64_t)(t * BK + (lane & (BK - 1))) * a.m_sk] : 0;
+  };
+  auto issue = [&](int t, int buf) {
+    const int k0 = t * BK, n = min(BK, len - k0);
+    const rsrc_t rk = rows_rsrc(kb + (int64_t)k0 * kp, n, kp, a.D * TL::ES);
+    const rsrc_t rv = rows_rsrc(vb + (int64_t)k0 * vp, n, vp, a.D * TL::ES);
+    uint64_t m = 0;
+    if constexpr (MASK == 1) m = __ballot(byte != 0);
 #pragma unroll
-      for (int j = 0; j < L::PER; ++j) {
-        const int r = L::row_of(tid, j);
-        const bool see = r < n && mk[(int64_t)(k0 + min(r, n - 1)) * a.m_sk] != 0;
-        raft_dma16(rs, at + j * 4096, see ? ld.off[j] : kOob);
-      }
-      if (keys && tid < BK) bias[buf][tid] = tid < n && mk[(int64_t)(k0 + min(tid, n - 1)) * a.m_sk] != 0 ? 0.f : -INFINITY;
-    } else {
-      ld.issue(rs, at);
+    for (int j = 0; j < Loader<T, DP, BK, 256>::PER; ++j) {
+      // (a hidden key's row is not fetched at all, whatever it holds)
+      const bool see = MASK != 1 || (m >> Loader<T, DP, BK, 256>::row_of(tid, j) & 1);
+      raft_dma16(rk, lds + 2 * buf * C::TILE + j * 4096, see ? lk.off[j] : kOob);
+      raft_dma16(rv, lds + (2 * buf + 1) * C::TILE + j * 4096, see ? lv.off[j] : kOob);
     }
+    if (t + 1 < t1) look(t + 1);
+    return m;
   };
   const uint32_t krow = TL::rows_base(raft_lds_addr(&kv[0][0][0]), lane), vcol = TL::cols_base(raft_lds_addr(&kv[0][1][0]), lane);
   const float c = a.scale_log2;
-  if (t0 < t1) issue(t0, true), issue(t0, false);
+  uint64_t next = 0;
+  if (t0 < t1) {
+    look(t0);
+    next = issue(t0, 0);
+  }
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1, k0 = t * BK;
     raft_wait_vmcnt<0>();
     __syncthreads();  // tile t has landed for all waves, and all have left tile t - 1's buffer
-    if (t + 1 < t1) issue(t + 1, true), issue(t + 1, false);
+    keys = next;
+    if (t + 1 < t1) next = issue(t + 1, buf ^ 1);
     if (k0 >= wlim) continue;
     f32x16 s[NB];
     st.scores(krow + buf * 2 * C::TILE, s);
     if (MASK || k0 + BK > wmin)
-      hide<NB, MASK>(s, lim - k0, hi, bias[buf], MASK == 2 ? mk + (int64_t)k0 * a.m_sk : nullptr, a.m_sk, a.Lk - k0);
+      hide<NB, MASK>(s, lim - k0, hi, keys, MASK == 2 ? mk + (int64_t)k0 * a.m_sk : nullptr, a.m_sk, a.Lk - k0);
     st.raise(s, c);
     st.probs(s, c);
     st.values(vcol + buf * 2 * C::TILE, s);
@@ -285,34 +290,42 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnArgs a) {
   const uint32_t krow = TL::rows_base(lds, lane), vcol = TL::cols_base(lds + TILE, lane);
   const uint8_t* mk = MASK ? a.mask + b * a.m_sb + (MASK == 2 ? h * a.m_sh + (int64_t)qi * a.m_sq : 0) : nullptr;
 
+  uint8_t byte = 0;
+  uint64_t keys = 0, next = 0;
+  auto look = [&](int t) {
+    if constexpr (MASK == 1) byte = row < len - t * 32 ? mk[(int64_t)(t * 32 + row) * a.m_sk] : 0;
+  };
   auto issue = [&](int t, int buf) {
     const int k0 = t * 32, n = min(32, len - k0);
     const rsrc_t rk = rows_rsrc(kb + (int64_t)k0 * kp, n, kp, a.D * TL::ES);
     const rsrc_t rv = rows_rsrc(vb + (int64_t)k0 * vp, n, vp, a.D * TL::ES);
-    if constexpr (MASK == 1) {
+    uint64_t m = 0;
+    if constexpr (MASK == 1) m = __ballot(byte != 0);
 #pragma unroll
-      for (int j = 0; j < L::PER; ++j) {
-        const int r = L::row_of(lane, j);
-        const bool see = r < n && mk[(int64_t)(k0 + min(r, n - 1)) * a.m_sk] != 0;
-        raft_dma16(rk, lds + (2 * buf) * TILE + j * 1024, see ? lk.off[j] : kOob);
-        raft_dma16(rv, lds + (2 * buf + 1) * TILE + j * 1024, see ? lv.off[j] : kOob);
-      }
-    } else {
-      lk.issue(rk, lds + (2 * buf) * TILE);
-      lv.issue(rv, lds + (2 * buf + 1) * TILE);
+    for (int j = 0; j < L::PER; ++j) {
+      const bool see = MASK != 1 || (m >> L::row_of(lane, j) & 1);
+      raft_dma16(rk, lds + 2 * buf * TILE + j * 1024, see ? lk.off[j] : kOob);
+      raft_dma16(rv, lds + (2 * buf + 1) * TILE + j * 1024, see ? lv.off[j] : kOob);
     }
+    if (t + 4 < t1) look(t + 4);
+    return m;
   };
 
   int t = t0 + wave;
-  if (BUFS == 2 && t < t1) issue(t, 0);
+  if (t < t1) look(t);
+  if (BUFS == 2 && t < t1) next = issue(t, 0);
   for (int buf = 0; t < t1; t += 4, buf ^= BUFS - 1) {
     const int k0 = t * 32;
     // the next block's DMA overwrites the buffer read two blocks ago: those reads have returned
     // (their products were issued), and the wait below leaves only the next block in flight
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    keys = next;
     if (BUFS == 1) {
-      issue(t, 0);
+      keys = issue(t, 0);
       raft_wait_vmcnt<0>();
+    } else if (MASK == 1) {
+      raft_wait_vmcnt<0>();  // (the look ahead is counted too)
+      if (t + 4 < t1) next = issue(t + 4, buf ^ 1);
     } else if (t + 4 < t1) {
       issue(t + 4, buf ^ 1);
       raft_wait_vmcnt<2 * L::PER>();
@@ -323,19 +336,8 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnArgs a) {
     asm volatile("" ::: "memory");
     f32x16 s[1];
     st.scores(krow + 2 * buf * TILE, s);
-    if (MASK || k0 + 32 > wmin) {
-      if constexpr (MASK == 1) {
-        const int64_t left = len - 1 - k0;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j = (r >> 2) * 8 + hi * 4 + (r & 3);
-          const bool see = j < lim - k0 && mk[(k0 + (j < left ? j : left)) * a.m_sk] != 0;
-          s[0][r] = see ? s[0][r] : -INFINITY;
-        }
-      } else {
-        hide<1, MASK>(s, lim - k0, hi, nullptr, MASK == 2 ? mk + (int64_t)k0 * a.m_sk : nullptr, a.m_sk, a.Lk - k0);
-      }
-    }
+    if (MASK || k0 + 32 > wmin)
+      hide<1, MASK>(s, lim - k0, hi, keys, MASK == 2 ? mk + (int64_t)k0 * a.m_sk : nullptr, a.m_sk, a.Lk - k0);
     st.raise(s, a.scale_log2);
     st.probs(s, a.scale_log2);
     st.values(vcol + 2 * buf * TILE, s);
