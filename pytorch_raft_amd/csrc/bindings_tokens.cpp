@@ -107,7 +107,7 @@ AttnArgs attn_args(const Tensor& q, const Tensor& k, const Tensor& v, double sca
   return a;
 }
 
-// -> {out (B, Lq, H, D), log2-sum-exp2 of the rows (B, Hkv, Lq * G) or empty}
+// -> {out (B, Lq, H, D), log2-sum-exp2 of the rows (B, Hkv, Lq * G) or empty, what out's rounding took away or empty}
 std::vector<Tensor> attn_fwd(const Tensor& q0, const Tensor& k0, const Tensor& v0, double scale, bool causal,
                              OptTensor mask, OptTensor lengths, OptTensor q_offset, bool need_lse) {
   TORCH_CHECK(q0.dim() == 4 && k0.dim() == 4 && v0.dim() == 4, "q must be (B, Lq, H, D), k and v (B, Lk, Hkv, D)");
@@ -118,10 +118,13 @@ std::vector<Tensor> attn_fwd(const Tensor& q0, const Tensor& k0, const Tensor& v
   const int64_t R = (int64_t)a.G * a.Lq;
   if (a.B == 0 || a.Lq == 0 || a.Lk == 0)
     return {at::zeros(q.sizes(), q.options()),
-            need_lse ? at::full({a.B, a.Hkv, R}, std::numeric_limits<float>::infinity(), f32) : at::empty({0}, f32)};
+            need_lse ? at::full({a.B, a.Hkv, R}, std::numeric_limits<float>::infinity(), f32) : at::empty({0}, f32), at::empty({0}, q.options())};
   Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
   Tensor lse = need_lse ? at::empty({a.B, a.Hkv, R}, f32) : at::empty({0}, f32);
+  const bool pair = need_lse && a.dtype != 2;
+  Tensor lo = pair ? at::empty_like(out) : at::empty({0}, q.options());
   a.o = out.data_ptr();
+  a.o_lo = pair ? lo.data_ptr() : nullptr;
   a.lse = need_lse ? lse.data_ptr<float>() : nullptr;
   attn_fwd_plan(a);
   Tensor part;
@@ -132,13 +135,13 @@ std::vector<Tensor> attn_fwd(const Tensor& q0, const Tensor& k0, const Tensor& v
     a.part_ml = a.part + n * a.DP;
   }
   launch_attn_fwd(a, cur_stream());
-  return {out, lse};
+  return {out, lse, lo};
 }
 
 // -> {dq, dk, dv}, contiguous
 std::vector<Tensor> attn_bwd(const Tensor& dout0, const Tensor& q0, const Tensor& k0, const Tensor& v0,
-                             const Tensor& out, const Tensor& lse, double scale, bool causal, OptTensor mask,
-                             OptTensor lengths, OptTensor q_offset) {
+                             const Tensor& out, const Tensor& lse, const Tensor& lo, double scale, bool causal,
+                             OptTensor mask, OptTensor lengths, OptTensor q_offset) {
   TORCH_CHECK(q0.dim() == 4 && k0.dim() == 4 && v0.dim() == 4, "q must be (B, Lq, H, D), k and v (B, Lk, Hkv, D)");
   c10::DeviceGuard g(q0.device());
   TORCH_CHECK(dout0.device() == q0.device() && dout0.scalar_type() == q0.scalar_type() && dout0.sizes() == q0.sizes(),
@@ -150,6 +153,8 @@ std::vector<Tensor> attn_bwd(const Tensor& dout0, const Tensor& q0, const Tensor
               "out must be the forward's");
   TORCH_CHECK(lse.device() == q.device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() && lse.numel() == (int64_t)a.B * a.Hkv * R,
               "lse must be the forward's");
+  TORCH_CHECK(lo.numel() == 0 || (lo.device() == q.device() && lo.scalar_type() == q.scalar_type() && lo.sizes() == q.sizes() && lo.is_contiguous()),
+              "lo must be the forward's");
   Tensor dq = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
   Tensor dk = at::empty(k.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
   Tensor dv = at::empty(k.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
@@ -162,6 +167,7 @@ std::vector<Tensor> attn_bwd(const Tensor& dout0, const Tensor& q0, const Tensor
   a.part = ws.data_ptr<float>();
   a.part_q = a.part + n_kv;
   a.o = out.data_ptr();
+  a.o_lo = lo.numel() ? lo.data_ptr() : nullptr;
   a.lse = lse.data_ptr<float>();
   a.dout = dout.data_ptr();
   a.d_sb = stride_of(dout, 0), a.d_sl = stride_of(dout, 1), a.d_sh = stride_of(dout, 2);
@@ -318,7 +324,7 @@ struct AttentionNode : public torch::autograd::Function<AttentionNode> {
     at::AutoDispatchBelowADInplaceOrView below;
     auto r = attn_fwd(q, k, v, scale, causal, mask, lengths, q_offset, true);
     const auto opt = [](OptTensor t) { return given(t) ? *t : Tensor(); };
-    ctx->save_for_backward({q, k, v, r[0], r[1], opt(mask), opt(lengths), opt(q_offset)});
+    ctx->save_for_backward({q, k, v, r[0], r[1], r[2], opt(mask), opt(lengths), opt(q_offset)});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["causal"] = causal;
     return r[0];
@@ -327,8 +333,8 @@ struct AttentionNode : public torch::autograd::Function<AttentionNode> {
     once_only("attention");
     const auto s = ctx->get_saved_variables();
     const auto opt = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
-    auto r = attn_bwd(grads[0], s[0], s[1], s[2], s[3], s[4], ctx->saved_data["scale"].toDouble(), ctx->saved_data["causal"].toBool(),
-                      opt(s[5]), opt(s[6]), opt(s[7]));
+    auto r = attn_bwd(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["scale"].toDouble(),
+                      ctx->saved_data["causal"].toBool(), opt(s[6]), opt(s[7]), opt(s[8]));
     return {r[0], r[1], r[2], Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
@@ -501,7 +507,7 @@ TORCH_LIBRARY_FRAGMENT(raft_amd, m) {
   m.def("rms_norm_int8(Tensor x, Tensor w, Tensor? residual, float eps) -> Tensor[]");
   m.def("int8_linear(Tensor x, Tensor xs, Tensor w, Tensor ws, Tensor? bias, int out_dtype) -> Tensor");
   m.def("attn_fwd(Tensor q, Tensor k, Tensor v, float scale, bool causal, Tensor? mask, Tensor? lengths, Tensor? q_offset, bool need_lse) -> Tensor[]");
-  m.def("attn_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, float scale, bool causal, Tensor? mask, Tensor? lengths, Tensor? q_offset) -> Tensor[]");
+  m.def("attn_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, Tensor lo, float scale, bool causal, Tensor? mask, Tensor? lengths, Tensor? q_offset) -> Tensor[]");
   m.def("rms_fwd(Tensor x, Tensor w, Tensor? residual, float eps, bool need_rstd) -> Tensor[]");
   m.def("rms_fwd_int8(Tensor x, Tensor w, Tensor? residual, float eps) -> Tensor[]");
   m.def("rms_bwd(Tensor dy, Tensor? dh, Tensor h, Tensor w, Tensor rstd) -> Tensor[]");

@@ -61,7 +61,9 @@ __device__ __forceinline__ float ds_scale(const AttnArgs& a) {
   }
 }
 
-// delta of every row; fp16: also the largest squared 2-norm of a dout row and of a v row that this
+// delta of every row, from the output as a pair of 16-bit values (rounded value and what the rounding
+// took away): where one key takes nearly all of a row, dP - delta cancels, and a delta from the rounded
+// output alone left errors in dq and dk of up to 2.5 times the rounding of the result.  fp16: also the largest squared 2-norm of a dout row and of a v row that this
 // block met, as float bits (ordered like the floats, NaN above all).  16 lanes of 8 channels a row.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_prep_kernel(AttnArgs a) {
@@ -76,11 +78,16 @@ __global__ __launch_bounds__(256) void attn_prep_kernel(AttnArgs a) {
       const int bh = (int)(w / R), row = (int)(w - (int64_t)bh * R);
       const int b = bh / a.Hkv, hk = bh - b * a.Hkv, qi = row / a.G, h = hk * a.G + row % a.G;
       if (d < a.D) {
-        const v8 o = *reinterpret_cast<const v8*>(reinterpret_cast<const T*>(a.o) + (((int64_t)b * a.Lq + qi) * a.Hkv * a.G + h) * a.D + d);
+        const int64_t at = (((int64_t)b * a.Lq + qi) * a.Hkv * a.G + h) * a.D + d;
+        const v8 o = *reinterpret_cast<const v8*>(reinterpret_cast<const T*>(a.o) + at);
+        v8 lo;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) lo[i] = (T)0.f;
+        if (a.o_lo) lo = *reinterpret_cast<const v8*>(reinterpret_cast<const T*>(a.o_lo) + at);
         const v8 g = *reinterpret_cast<const v8*>(reinterpret_cast<const T*>(a.dout) + b * a.d_sb + qi * a.d_sl + h * a.d_sh + d);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          s = fmaf((float)g[i], (float)o[i], s);
+          s = fmaf((float)g[i], (float)o[i] + (float)lo[i], s);
           n = fmaf((float)g[i], (float)g[i], n);
         }
       }

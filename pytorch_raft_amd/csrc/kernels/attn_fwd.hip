@@ -119,9 +119,10 @@ __device__ __forceinline__ void hide(f32x16 (&s)[NB], int left, int hi, uint64_t
   }
 }
 
-// lane's output row (column of O^T): 4 consecutive channels per 4 registers
+// lane's output row (column of O^T): 4 consecutive channels per 4 registers.  lo (training): what the
+// rounding took away, for the backward's row sums.
 template <typename T, int DB>
-__device__ __forceinline__ void store_row(T* p, const f32x16 (&o)[DB], float f, int D, int hi) {
+__device__ __forceinline__ void store_row(T* p, T* lo, const f32x16 (&o)[DB], float f, int D, int hi) {
 #pragma unroll
   for (int i = 0; i < DB; ++i)
 #pragma unroll
@@ -129,10 +130,14 @@ __device__ __forceinline__ void store_row(T* p, const f32x16 (&o)[DB], float f, 
       const int d = i * 32 + g * 8 + hi * 4;
       if (d < D) {
         typedef T v4 __attribute__((ext_vector_type(4)));
-        v4 w;
+        v4 w, x;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = (T)(o[i][4 * g + k] * f);
+        for (int k = 0; k < 4; ++k) {
+          w[k] = (T)(o[i][4 * g + k] * f);
+          x[k] = (T)(o[i][4 * g + k] * f - (float)w[k]);
+        }
         *reinterpret_cast<v4*>(p + d) = w;
+        if (lo) *reinterpret_cast<v4*>(lo + d) = x;
       }
     }
 }
@@ -231,14 +236,15 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
   if (!ok) return;
   if (a.nsplit > 1) {
     const int64_t p = ((int64_t)bh * a.nsplit + split) * R + row;
-    store_row<float>(a.part + p * DP, st.o, 1.f, DP, hi);
+    store_row<float>(a.part + p * DP, nullptr, st.o, 1.f, DP, hi);
     if (hi == 0) {
       a.part_ml[2 * p] = st.m;
       a.part_ml[2 * p + 1] = l;
     }
     return;
   }
-  store_row<T>(reinterpret_cast<T*>(a.o) + (((int64_t)b * a.Lq + qi) * a.Hkv * a.G + h) * a.D, st.o,
+  const int64_t at = (((int64_t)b * a.Lq + qi) * a.Hkv * a.G + h) * a.D;
+  store_row<T>(reinterpret_cast<T*>(a.o) + at, a.o_lo ? reinterpret_cast<T*>(a.o_lo) + at : nullptr, st.o,
                l > 0.f || l != l ? 1.f / l : 0.f, a.D, hi);
   if (a.lse && hi == 0) a.lse[(int64_t)bh * R + row] = l > 0.f || l != l ? st.m + log2f(l) : INFINITY;
 }
@@ -359,7 +365,7 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnArgs a) {
   for (int w = 0; w < 4; ++w) lt += ml[w][row][1] * __builtin_amdgcn_exp2f(ml[w][row][0] - ms);
   const float f = __builtin_amdgcn_exp2f(st.m - ms);
   float* jo = reinterpret_cast<float*>(sm);
-  store_row<float>(jo + (wave * 32 + row) * (DP + 4), st.o, f, DP, hi);
+  store_row<float>(jo + (wave * 32 + row) * (DP + 4), nullptr, st.o, f, DP, hi);
   __syncthreads();
   const bool some = lt > 0.f || lt != lt;
   if (a.nsplit == 1 && a.lse && wave == 0 && hi == 0 && ok) a.lse[(int64_t)bh * R + row] = some ? mt + log2f(lt) : INFINITY;
@@ -380,7 +386,10 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnArgs a) {
       a.part[(((int64_t)bh * a.nsplit + split) * R + r) * DP + d] = v;
     } else if (d < a.D) {
       const int q2 = r / a.G, g2 = r - q2 * a.G;
-      reinterpret_cast<T*>(a.o)[(((int64_t)b * a.Lq + q2) * a.Hkv * a.G + hk * a.G + g2) * a.D + d] = (T)(v * ml[0][r][0]);
+      const int64_t at = (((int64_t)b * a.Lq + q2) * a.Hkv * a.G + hk * a.G + g2) * a.D + d;
+      const T w = (T)(v * ml[0][r][0]);
+      reinterpret_cast<T*>(a.o)[at] = w;
+      if (a.o_lo) reinterpret_cast<T*>(a.o_lo)[at] = (T)(v * ml[0][r][0] - (float)w);
     }
   }
 }
@@ -394,28 +403,36 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   const int lane = threadIdx.x & 63;
   const int bh = (int)(w / R), row = (int)(w - (int64_t)bh * R);
   const int64_t p0 = (int64_t)bh * a.nsplit * R + row;
-  float mt = -INFINITY;
-  for (int s = 0; s < a.nsplit; ++s) mt = fmaxf(mt, a.part_ml[2 * (p0 + (int64_t)s * R)]);
-  const float ms = mt == -INFINITY ? 0.f : mt;
+  // lane s: the s-th range's maximum, sum and factor (at most 64 ranges)
+  const bool mine = lane < a.nsplit;
+  const float m = mine ? a.part_ml[2 * (p0 + (int64_t)lane * R)] : -INFINITY;
+  float mt = m;
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) mt = fmaxf(mt, __shfl_xor(mt, x, 64));
+  const float fs = __builtin_amdgcn_exp2f(m - (mt == -INFINITY ? 0.f : mt));
+  const float lt = wave_sum(mine ? a.part_ml[2 * (p0 + (int64_t)lane * R) + 1] * fs : 0.f);
   constexpr int PL = (DP + 63) / 64;
-  float lt = 0.f, o[PL];
+  float o[PL];
 #pragma unroll
   for (int k = 0; k < PL; ++k) o[k] = 0.f;
+#pragma unroll 8
   for (int s = 0; s < a.nsplit; ++s) {
-    const int64_t p = p0 + (int64_t)s * R;
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * p] - ms);
-    lt += a.part_ml[2 * p + 1] * f;
+    const float f = __shfl(fs, s, 64);
 #pragma unroll
     for (int k = 0; k < PL; ++k)
-      if (lane + 64 * k < DP) o[k] += a.part[p * DP + lane + 64 * k] * f;
+      if (lane + 64 * k < DP) o[k] += a.part[(p0 + (int64_t)s * R) * DP + lane + 64 * k] * f;
   }
   const bool some = lt > 0.f || lt != lt;
   const float inv = some ? 1.f / lt : 0.f;
   const int b = bh / a.Hkv, hk = bh - b * a.Hkv, qi = row / a.G, g = row - qi * a.G;
-  T* out = reinterpret_cast<T*>(a.o) + (((int64_t)b * a.Lq + qi) * a.Hkv * a.G + hk * a.G + g) * a.D;
+  const int64_t at = (((int64_t)b * a.Lq + qi) * a.Hkv * a.G + hk * a.G + g) * a.D;
 #pragma unroll
   for (int k = 0; k < PL; ++k)
-    if (lane + 64 * k < a.D) out[lane + 64 * k] = (T)(o[k] * inv);
+    if (lane + 64 * k < a.D) {
+      const T w = (T)(o[k] * inv);
+      reinterpret_cast<T*>(a.o)[at + lane + 64 * k] = w;
+      if (a.o_lo) reinterpret_cast<T*>(a.o_lo)[at + lane + 64 * k] = (T)(o[k] * inv - (float)w);
+    }
   if (a.lse && lane == 0) a.lse[(int64_t)bh * R + row] = some ? mt + log2f(lt) : INFINITY;
 }
 

@@ -459,7 +459,7 @@ bool launch_image_prep(const float* a, const float* b, void* out, int B, int64_t
 // (B, Hkv, G * Lq) in log2 units / fp32, rows position-major over the G heads of a key head.
 struct AttnArgs {
   const void *q, *k, *v;
-  void* o;
+  void *o, *o_lo;         // o_lo: what o's rounding took away (16-bit types, training; else null)
   float* lse;             // nullable in the forward
   int64_t q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh;
   int B, Lq, Lk, Hkv, G, D, DP;

@@ -218,6 +218,7 @@ __global__ __launch_bounds__(1024) void rms_dw_kernel(RmsArgs a) {
   const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
   float s = 0.f;
   if (c < a.C)
+#pragma unroll 8
     for (int p = k; p < a.parts; p += 32) s += a.part[(int64_t)p * a.C + c];
   sh[k][threadIdx.x & 31] = s;
   __syncthreads();
