@@ -134,6 +134,11 @@ std::vector<Tensor> attn_fwd(const Tensor& q0, const Tensor& k0, const Tensor& v
     a.part = part.data_ptr<float>();
     a.part_ml = a.part + n * a.DP;
   }
+  Tensor bits;
+  if (const int64_t n = attn_bit_words(a, false)) {
+    bits = at::empty({n}, q.options().dtype(at::kLong));
+    a.row_bits = reinterpret_cast<uint64_t*>(bits.data_ptr<int64_t>());
+  }
   launch_attn_fwd(a, cur_stream());
   return {out, lse, lo};
 }
@@ -176,6 +181,12 @@ std::vector<Tensor> attn_bwd(const Tensor& dout0, const Tensor& q0, const Tensor
   a.dq = dq.data_ptr();
   a.dk = dk.data_ptr();
   a.dv = dv.data_ptr();
+  Tensor bits;
+  if (const int64_t n = attn_bit_words(a, false)) {
+    bits = at::empty({n + attn_bit_words(a, true)}, q.options().dtype(at::kLong));
+    a.row_bits = reinterpret_cast<uint64_t*>(bits.data_ptr<int64_t>());
+    a.key_bits = a.row_bits + n;
+  }
   launch_attn_bwd(a, cur_stream());
   return {dq, dk, dv};
 }

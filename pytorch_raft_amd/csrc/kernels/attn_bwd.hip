@@ -282,7 +282,7 @@ __device__ __forceinline__ void dkv_body(const AttnArgs& a, int bid, int grid, u
       dp = mma(AHEAD ? fd[i] : TL::rows(qrow + at + TILE, hb, i), vf[i], dp);
     }
   };
-  auto weights = [&](auto edge, f32x16& s, f32x16& dp, int row0, const float* st) {
+  auto weights = [&](auto edge, f32x16& s, f32x16& dp, int row0, const float* st, uint32_t bits) {
 #pragma unroll
     for (int r4 = 0; r4 < 4; ++r4) {
       const f32x4 ls = *reinterpret_cast<const f32x4*>(st + r4 * 8 + hi * 4);
@@ -301,11 +301,7 @@ __device__ __forceinline__ void dkv_body(const AttnArgs& a, int bid, int grid, u
       for (int r = 0; r < 16; ++r) {
         const int row = row0 + (r >> 2) * 8 + hi * 4 + (r & 3);
         bool on = !a.causal || key <= off + row / a.G;
-        if constexpr (MASK == 2) {
-          const int rr = min(row, R - 1), qi = rr / a.G;
-          on = on && a.mask[b * a.m_sb + (int64_t)(hk * a.G + rr - qi * a.G) * a.m_sh + (int64_t)qi * a.m_sq +
-                            (int64_t)min(key, a.Lk - 1) * a.m_sk] != 0;
-        }
+        if constexpr (MASK == 2) on = on && (bits >> ((r >> 2) * 8 + hi * 4 + (r & 3)) & 1);
         s[r] = on ? s[r] : 0.f;
         dp[r] = on ? dp[r] : 0.f;
       }
@@ -322,7 +318,7 @@ __device__ __forceinline__ void dkv_body(const AttnArgs& a, int bid, int grid, u
       }
     }
   };
-  auto walk = [&](auto edge, int row0, uint32_t at, const float* st, uint32_t at_next) {
+  auto walk = [&](auto edge, int row0, uint32_t at, const float* st, uint32_t at_next, uint64_t bits) {
     if constexpr (NB == 2) {
       f32x16 s0, p0, s1, p1;
       products(s0, p0, at, 0);
@@ -330,11 +326,11 @@ __device__ __forceinline__ void dkv_body(const AttnArgs& a, int bid, int grid, u
       pin<2 * DT, 1>();
       products(s1, p1, at, 1);
       load_cols(at, 0);
-      weights(edge, s0, p0, row0, st);
+      weights(edge, s0, p0, row0, st, (uint32_t)bits);
       pin<2 * DT, 2>();
       gradients(s0, p0, at, 0);
       load_cols(at, 1);
-      weights(edge, s1, p1, row0 + 32, st + 32);
+      weights(edge, s1, p1, row0 + 32, st + 32, (uint32_t)(bits >> 32));
       pin<2 * DT, 2>();
       gradients(s1, p1, at, 1);
       load_rows(at_next, 0);
@@ -342,18 +338,23 @@ __device__ __forceinline__ void dkv_body(const AttnArgs& a, int bid, int grid, u
     } else {
       f32x16 s, dp;
       products(s, dp, at, 0);
-      weights(edge, s, dp, row0, st);
+      weights(edge, s, dp, row0, st, (uint32_t)bits);
       gradients(s, dp, at, 0);
     }
   };
   // three buffers: tile t + 1 has landed when tile t begins, for the last block's look ahead
   uint32_t b0 = 0, b1 = 2 * TILE, b2 = 4 * TILE;
   int s0 = 0, s1 = 2 * BT, s2 = 4 * BT;
+  // mask: this key's bits over the rows of a tile, looked up a tile ahead
+  const uint64_t* mw = MASK == 2 ? key_bits(a, b, hk, min(key, a.Lk - 1)) : nullptr;
+  uint64_t word = MASK == 2 && t0 < t1 ? mw[t0 * BT / 64] >> (t0 * BT % 64) : 0;
   auto turn = [&](auto edge, int t) {
     raft_wait_vmcnt<0>();
     __syncthreads();  // tile t + 1 has landed for all waves, and all have left tile t - 1
     if (t + 2 < t1) issue(t + 2, b2, s2);
-    walk(edge, t * BT, b0, stat + s0, b1);
+    const uint64_t bits = word;
+    if constexpr (MASK == 2) word = t + 1 < t1 ? mw[(t + 1) * BT / 64] >> ((t + 1) * BT % 64) : 0;
+    walk(edge, t * BT, b0, stat + s0, b1, bits);
     const uint32_t x = b0;
     b0 = b1, b1 = b2, b2 = x;
     const int y = s0;
@@ -438,19 +439,20 @@ __device__ __forceinline__ void dq_body(const AttnArgs& a, int bid, int grid, ui
   lv.init(tid, vp, a.D * TL::ES);
   const uint32_t lds = raft_lds_addr(sm) + wave * 1024;
   const uint32_t krow = TL::rows_base(raft_lds_addr(sm), lane), kcol = TL::cols_base(raft_lds_addr(sm), lane);
-  const uint8_t* mk = MASK ? a.mask + b * a.m_sb + (MASK == 2 ? h * a.m_sh + (int64_t)qi * a.m_sq : 0) : nullptr;
+  const uint8_t* mk = MASK == 1 ? a.mask + b * a.m_sb : nullptr;
+  const uint64_t* mw = MASK == 2 ? row_bits(a, b, hk, rc) : nullptr;
 
-  uint8_t byte = 0;  // key mask: the next tile's bytes, and the seen keys of three tiles as bits
-  uint64_t m0 = 0, m1 = 0, m2 = 0;
+  uint8_t byte = 0;  // masks: looked up a tile ahead; the bits of three tiles
+  uint64_t word = 0, m0 = 0, m1 = 0, m2 = 0;
   auto look = [&](int t) {
+    if constexpr (MASK == 2) word = mw[t * BK / 64] >> (t * BK % 64);
     if constexpr (MASK == 1) byte = (lane & (BK - 1)) < len - t * BK ? mk[(int64_t)(t * BK + (lane & (BK - 1))) * a.m_sk] : 0;
   };
   auto issue = [&](int t, uint32_t buf) {
     const int k0 = t * BK, n = min(BK, len - k0);
     const rsrc_t rk = rows_rsrc(kb + (int64_t)k0 * kp, n, kp, a.D * TL::ES);
     const rsrc_t rv = rows_rsrc(vb + (int64_t)k0 * vp, n, vp, a.D * TL::ES);
-    uint64_t m = 0;
-    if constexpr (MASK == 1) m = __ballot(byte != 0);
+    const uint64_t m = MASK == 1 ? __ballot(byte != 0) : word;
 #pragma unroll
     for (int j = 0; j < L::PER; ++j) {
       const bool see = MASK != 1 || (m >> L::row_of(tid, j) & 1);
@@ -495,8 +497,7 @@ __device__ __forceinline__ void dq_body(const AttnArgs& a, int bid, int grid, ui
       for (int r = 0; r < 16; ++r) {
         const int j = (r >> 2) * 8 + hi * 4 + (r & 3);
         bool on = k0 + j < lim;
-        if constexpr (MASK == 1) on = on && (keys >> j & 1);
-        if constexpr (MASK == 2) on = on && mk[(int64_t)min(k0 + j, a.Lk - 1) * a.m_sk] != 0;
+        if constexpr (MASK != 0) on = on && (keys >> j & 1);
         s[r] = on ? s[r] : 0.f;
       }
     }
@@ -594,6 +595,7 @@ __global__ __launch_bounds__(256) void attn_grad_join_kernel(AttnArgs a, int64_t
 template <typename T, int DP, int MASK>
 void bwd_launch(const AttnArgs& a, hipStream_t s) {
   const int64_t R = (int64_t)a.G * a.Lq, heads = (int64_t)a.B * a.Hkv;
+  if (a.mask_mode == 2) launch_attn_pack(a, s);
   attn_prep_kernel<T><<<a.nprep, 256, 0, s>>>(a);
   const int gk = (int)raft_cdiv((int64_t)raft_cdiv(a.Lk, 128) * heads * a.nsplit_kv, 8) * 8;
   const int gq = (int)raft_cdiv((int64_t)raft_cdiv(R, 128) * heads * a.nsplit_q, 8) * 8;

@@ -210,4 +210,17 @@ __device__ __forceinline__ int item_off(const AttnArgs& a, int b) {
   return a.q_offset ? max(-a.Lq, min(a.q_offset[b], a.Lk)) : a.Lk - a.Lq;
 }
 
+// A (query, key) mask comes as bits, packed once a call by attn_pack_kernel: for each row (packed order)
+// words over 64 keys, and for the dk / dv kernel for each key words over 64 rows.  Masks shared by heads
+// or items are packed once (bit_head).
+__device__ __forceinline__ int64_t bit_head(const AttnArgs& a, int b, int hk) {
+  return (a.m_sb ? (int64_t)b * (a.m_sh ? a.Hkv : 1) : 0) + (a.m_sh ? hk : 0);
+}
+__device__ __forceinline__ const uint64_t* row_bits(const AttnArgs& a, int b, int hk, int row) {
+  return a.row_bits + (bit_head(a, b, hk) * a.G * a.Lq + row) * ((a.Lk + 63) / 64);
+}
+__device__ __forceinline__ const uint64_t* key_bits(const AttnArgs& a, int b, int hk, int key) {
+  return a.key_bits + (bit_head(a, b, hk) * a.Lk + key) * ((a.G * a.Lq + 63) / 64);
+}
+
 }  // namespace attn_detail

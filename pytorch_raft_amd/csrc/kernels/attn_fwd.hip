@@ -101,19 +101,16 @@ struct RowState {
   }
 };
 
-// keys from `left` on (this lane's row) and keys hidden by the mask -> -inf.  keys: bits of the tile's
-// seen keys (key mask); full: this row's bytes of a (query, key) mask at the tile's first key.
+// keys from `left` on (this lane's row) and keys that the mask's bits for the tile leave out -> -inf
 template <int NB, int MASK>
-__device__ __forceinline__ void hide(f32x16 (&s)[NB], int left, int hi, uint64_t keys, const uint8_t* full, int64_t msk, int nkeys) {
+__device__ __forceinline__ void hide(f32x16 (&s)[NB], int left, int hi, uint64_t keys) {
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     const uint32_t bits = (uint32_t)(keys >> (32 * b)) >> (4 * hi);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int j = b * 32 + (r >> 2) * 8 + hi * 4 + (r & 3);
-      bool see = j < left;
-      if constexpr (MASK == 1) see = see && (bits >> ((r >> 2) * 8 + (r & 3)) & 1);
-      if constexpr (MASK == 2) see = see && j < nkeys && full[min(j, nkeys - 1) * msk] != 0;
+      bool see = b * 32 + (r >> 2) * 8 + hi * 4 + (r & 3) < left;
+      if constexpr (MASK != 0) see = see && (bits >> ((r >> 2) * 8 + (r & 3)) & 1);
       s[b][r] = see ? s[b][r] : -INFINITY;
     }
   }
@@ -185,20 +182,21 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
   lk.init(tid, kp, a.D * TL::ES);
   lv.init(tid, vp, a.D * TL::ES);
   const uint32_t lds = raft_lds_addr(&kv[0][0][0]) + wave * 1024;
-  const uint8_t* mk = MASK ? a.mask + b * a.m_sb + (MASK == 2 ? h * a.m_sh + (int64_t)qi * a.m_sq : 0) : nullptr;
+  const uint8_t* mk = MASK == 1 ? a.mask + b * a.m_sb : nullptr;
+  const uint64_t* mw = MASK == 2 ? row_bits(a, b, hk, min(row, R - 1)) : nullptr;
 
-  // key mask: each wave looks a tile ahead at the tile's bytes and keeps them as bits
+  // masks: looked up a tile ahead; a key mask's bytes become bits by a ballot
   uint8_t byte = 0;
-  uint64_t keys = 0;
+  uint64_t word = 0, keys = 0;
   auto look = [&](int t) {
+    if constexpr (MASK == 2) word = mw[t * BK / 64] >> (t * BK % 64);
     if constexpr (MASK == 1) byte = (lane & (BK - 1)) < len - t * BK ? mk[(int64_t)(t * BK + (lane & (BK - 1))) * a.m_sk] : 0;
   };
   auto issue = [&](int t, int buf) {
     const int k0 = t * BK, n = min(BK, len - k0);
     const rsrc_t rk = rows_rsrc(kb + (int64_t)k0 * kp, n, kp, a.D * TL::ES);
     const rsrc_t rv = rows_rsrc(vb + (int64_t)k0 * vp, n, vp, a.D * TL::ES);
-    uint64_t m = 0;
-    if constexpr (MASK == 1) m = __ballot(byte != 0);
+    const uint64_t m = MASK == 1 ? __ballot(byte != 0) : word;
 #pragma unroll
     for (int j = 0; j < Loader<T, DP, BK, 256>::PER; ++j) {
       // (a hidden key's row is not fetched at all, whatever it holds)
@@ -226,7 +224,7 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     f32x16 s[NB];
     st.scores(krow + buf * 2 * C::TILE, s);
     if (MASK || k0 + BK > wmin)
-      hide<NB, MASK>(s, lim - k0, hi, keys, MASK == 2 ? mk + (int64_t)k0 * a.m_sk : nullptr, a.m_sk, a.Lk - k0);
+      hide<NB, MASK>(s, lim - k0, hi, keys);
     st.raise(s, c);
     st.probs(s, c);
     st.values(vcol + buf * 2 * C::TILE, s);
@@ -294,19 +292,20 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnArgs a) {
   lv.init(lane, vp, a.D * TL::ES);
   const uint32_t lds = raft_lds_addr(sm) + wave * 2 * BUFS * TILE;
   const uint32_t krow = TL::rows_base(lds, lane), vcol = TL::cols_base(lds + TILE, lane);
-  const uint8_t* mk = MASK ? a.mask + b * a.m_sb + (MASK == 2 ? h * a.m_sh + (int64_t)qi * a.m_sq : 0) : nullptr;
+  const uint8_t* mk = MASK == 1 ? a.mask + b * a.m_sb : nullptr;
+  const uint64_t* mw = MASK == 2 ? row_bits(a, b, hk, min(row, R - 1)) : nullptr;
 
   uint8_t byte = 0;
-  uint64_t keys = 0, next = 0;
+  uint64_t word = 0, keys = 0, next = 0;
   auto look = [&](int t) {
+    if constexpr (MASK == 2) word = mw[t / 2] >> (t % 2 * 32);
     if constexpr (MASK == 1) byte = row < len - t * 32 ? mk[(int64_t)(t * 32 + row) * a.m_sk] : 0;
   };
   auto issue = [&](int t, int buf) {
     const int k0 = t * 32, n = min(32, len - k0);
     const rsrc_t rk = rows_rsrc(kb + (int64_t)k0 * kp, n, kp, a.D * TL::ES);
     const rsrc_t rv = rows_rsrc(vb + (int64_t)k0 * vp, n, vp, a.D * TL::ES);
-    uint64_t m = 0;
-    if constexpr (MASK == 1) m = __ballot(byte != 0);
+    const uint64_t m = MASK == 1 ? __ballot(byte != 0) : word;
 #pragma unroll
     for (int j = 0; j < L::PER; ++j) {
       const bool see = MASK != 1 || (m >> L::row_of(lane, j) & 1);
@@ -329,7 +328,7 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnArgs a) {
     if (BUFS == 1) {
       keys = issue(t, 0);
       raft_wait_vmcnt<0>();
-    } else if (MASK == 1) {
+    } else if (MASK != 0) {
       raft_wait_vmcnt<0>();  // (the look ahead is counted too)
       if (t + 4 < t1) next = issue(t + 4, buf ^ 1);
     } else if (t + 4 < t1) {
@@ -343,7 +342,7 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnArgs a) {
     f32x16 s[1];
     st.scores(krow + 2 * buf * TILE, s);
     if (MASK || k0 + 32 > wmin)
-      hide<1, MASK>(s, lim - k0, hi, keys, MASK == 2 ? mk + (int64_t)k0 * a.m_sk : nullptr, a.m_sk, a.Lk - k0);
+      hide<1, MASK>(s, lim - k0, hi, keys);
     st.raise(s, a.scale_log2);
     st.probs(s, a.scale_log2);
     st.values(vcol + 2 * buf * TILE, s);
@@ -436,6 +435,29 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   if (a.lse && lane == 0) a.lse[(int64_t)bh * R + row] = some ? mt + log2f(lt) : INFINITY;
 }
 
+// A wave per 64 rows x 64 keys: a row's bytes become its word by a ballot, a lane collects its key's.
+__global__ __launch_bounds__(256) void attn_pack_kernel(AttnArgs a) {
+  const int R = a.G * a.Lq, nrt = (R + 63) / 64, nkt = (a.Lk + 63) / 64, nh = a.m_sh ? a.Hkv : 1, nb = a.m_sb ? a.B : 1;
+  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (w >= (int64_t)nb * nh * nrt * nkt) return;
+  const int lane = threadIdx.x & 63;
+  const int kt = (int)(w % nkt), rt = (int)(w / nkt % nrt), hk = (int)(w / nkt / nrt % nh), b = (int)(w / nkt / nrt / nh);
+  const int key = kt * 64 + lane;
+  const uint8_t* p = a.mask + b * a.m_sb + (int64_t)min(key, a.Lk - 1) * a.m_sk;
+  uint64_t mine = 0, col = 0;
+#pragma unroll 16
+  for (int i = 0; i < 64; ++i) {
+    const int row = rt * 64 + i, rc = min(row, R - 1), qi = rc / a.G, h = hk * a.G + rc - qi * a.G;
+    const bool see = row < R && key < a.Lk && p[h * a.m_sh + (int64_t)qi * a.m_sq] != 0;
+    const uint64_t bits = __ballot(see);
+    if (lane == i) mine = bits;
+    col |= (uint64_t)see << i;
+  }
+  const int64_t head = (int64_t)b * nh + hk;
+  if (rt * 64 + lane < R) a.row_bits[(head * R + rt * 64 + lane) * nkt + kt] = mine;
+  if (a.key_bits && key < a.Lk) a.key_bits[(head * a.Lk + key) * nrt + rt] = col;
+}
+
 template <typename T, int DP, int MASK>
 void fwd_launch(const AttnArgs& a, hipStream_t s) {
   const int64_t R = (int64_t)a.G * a.Lq;
@@ -471,7 +493,19 @@ void attn_fwd_plan(AttnArgs& a) {
   a.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(s, 64));
 }
 
+int64_t attn_bit_words(const AttnArgs& a, bool keys) {
+  if (a.mask_mode != 2) return 0;
+  const int64_t R = (int64_t)a.G * a.Lq, heads = (int64_t)(a.m_sb ? a.B : 1) * (a.m_sh ? a.Hkv : 1);
+  return heads * (keys ? a.Lk * ((R + 63) / 64) : R * ((a.Lk + 63) / 64));
+}
+
+void launch_attn_pack(const AttnArgs& a, hipStream_t s) {
+  const int64_t R = (int64_t)a.G * a.Lq, heads = (int64_t)(a.m_sb ? a.B : 1) * (a.m_sh ? a.Hkv : 1);
+  attn_detail::attn_pack_kernel<<<raft_cdiv(heads * ((R + 63) / 64) * ((a.Lk + 63) / 64), 4), 256, 0, s>>>(a);
+}
+
 void launch_attn_fwd(const AttnArgs& a, hipStream_t s) {
+  if (a.mask_mode == 2) launch_attn_pack(a, s);
   if (a.dtype == 0) attn_detail::fwd_dim<__bf16>(a, s);
   else if (a.dtype == 1) attn_detail::fwd_dim<_Float16>(a, s);
   else attn_detail::fwd_dim<float>(a, s);

@@ -470,6 +470,7 @@ struct AttnArgs {
   const uint8_t* mask;    // nonzero = seen; mode 0 none, 1 over keys (b, key), 2 over (b, h, query, key)
   int mask_mode;
   int64_t m_sb, m_sh, m_sq, m_sk;
+  uint64_t *row_bits, *key_bits;  // mode 2: packed mask, attn_bit_words of each (key_bits: backward)
   int nsplit;             // key ranges; > 1: partial outputs (B, Hkv, nsplit, R, DP) and (.., 2) max / sum
   float *part, *part_ml;
   // backward
@@ -483,6 +484,8 @@ struct AttnArgs {
   void *dq, *dk, *dv;     // contiguous (B, L, heads, D)
 };
 void attn_fwd_plan(AttnArgs& a);  // nsplit
+int64_t attn_bit_words(const AttnArgs& a, bool keys);  // 64-bit words of row_bits / key_bits
+void launch_attn_pack(const AttnArgs& a, hipStream_t s);
 void launch_attn_fwd(const AttnArgs& a, hipStream_t s);
 void attn_bwd_plan(AttnArgs& a);  // nprep, nsplit_kv, nsplit_q
 void launch_attn_bwd(const AttnArgs& a, hipStream_t s);
