@@ -194,16 +194,16 @@ std::vector<Tensor> attn_bwd(const Tensor& dout0, const Tensor& q0, const Tensor
 // ------------------------------------------------------------------ root-mean-square norm
 RmsArgs rms_args(const Tensor& x, const Tensor& w, double eps) {
   TORCH_CHECK(x.is_cuda() && w.device() == x.device(), "x and weight must be on one GPU");
-  TORCH_CHECK(x.dim() == 2 && x.is_contiguous(), "x must be contiguous (rows, C)");
-  TORCH_CHECK(x.size(1) >= 1 && x.size(1) <= 16384, "rms norm takes 1 to 16384 channels, got ", x.size(1));
-  TORCH_CHECK(w.dim() == 1 && w.size(0) == x.size(1) && w.is_contiguous() &&
+  TORCH_CHECK(x.dim() >= 1 && x.is_contiguous(), "x must be contiguous (..., C)");
+  TORCH_CHECK(x.size(-1) >= 1 && x.size(-1) <= 16384, "rms norm takes 1 to 16384 channels, got ", x.size(-1));
+  TORCH_CHECK(w.dim() == 1 && w.size(0) == x.size(-1) && w.is_contiguous() &&
                   (w.scalar_type() == at::kFloat || w.scalar_type() == x.scalar_type()),
               "weight must be contiguous (C,), float32 or the dtype of x");
   TORCH_CHECK(std::isfinite(eps) && eps >= 0, "eps must be finite and not negative");
   RmsArgs a = {};
   a.dtype = dtype_code(x, "x");
-  a.rows = x.size(0);
-  a.C = (int)x.size(1);
+  a.rows = x.numel() / x.size(-1);
+  a.C = (int)x.size(-1);
   a.eps = (float)eps;
   a.w = w.data_ptr();
   a.w_f32 = w.scalar_type() == at::kFloat;
@@ -221,7 +221,7 @@ std::vector<Tensor> rms_fwd(const Tensor& x, const Tensor& w, OptTensor residual
   c10::DeviceGuard g(x.device());
   const auto f32 = x.options().dtype(at::kFloat);
   Tensor y = at::empty_like(x), h = given(residual) ? at::empty_like(x) : at::empty({0}, x.options());
-  Tensor rstd = at::empty({need_rstd ? x.size(0) : 0}, f32);
+  Tensor rstd = at::empty({need_rstd ? a.rows : 0}, f32);
   if (given(residual)) {
     check_like(*residual, x, "residual");
     a.r = residual->data_ptr();
@@ -238,7 +238,7 @@ std::vector<Tensor> rms_fwd_int8(const Tensor& x, const Tensor& w, OptTensor res
   RmsArgs a = rms_args(x, w, eps);
   c10::DeviceGuard g(x.device());
   Tensor q = at::empty(x.sizes(), x.options().dtype(at::kChar)), h = given(residual) ? at::empty_like(x) : at::empty({0}, x.options());
-  Tensor scale = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
+  Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
   if (given(residual)) {
     check_like(*residual, x, "residual");
     a.r = residual->data_ptr();
@@ -255,7 +255,7 @@ std::vector<Tensor> rms_bwd(const Tensor& dy, OptTensor dh, const Tensor& h, con
   RmsArgs a = rms_args(h, w, 0.0);
   c10::DeviceGuard g(h.device());
   check_like(dy, h, "dy");
-  TORCH_CHECK(rstd.device() == h.device() && rstd.scalar_type() == at::kFloat && rstd.is_contiguous() && rstd.dim() == 1 && rstd.size(0) == h.size(0),
+  TORCH_CHECK(rstd.device() == h.device() && rstd.scalar_type() == at::kFloat && rstd.is_contiguous() && rstd.numel() == a.rows,
               "rstd must be the forward's");
   if (given(dh)) check_like(*dh, h, "dh");
   Tensor dx = at::empty_like(h), dw = at::empty_like(w);
@@ -288,7 +288,7 @@ Tensor int8_mm(const Tensor& x, const Tensor& xs, const Tensor& w, const Tensor&
   TORCH_CHECK(out_dtype >= 0 && out_dtype <= 2, "out_dtype: 0 bf16, 1 fp16, 2 fp32");
   const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
   TORCH_CHECK(K <= 131071, "int8_mm: K past 131071 could overflow the 32-bit sums");
-  TORCH_CHECK(M < (int64_t(1) << 28) && N < (int64_t(1) << 28) && ((M + 63) / 64) * ((N + 63) / 64) < (int64_t(1) << 23),
+  TORCH_CHECK(M < (int64_t(1) << 28) && N < (int64_t(1) << 26) && ((M + 63) / 64) * ((N + 63) / 64) < (int64_t(1) << 23),
               "int8_mm: too many outputs for one call");
   check_vec(xs, x, M, "xs");
   check_vec(ws, x, N, "ws");
@@ -416,20 +416,13 @@ void rms_check(const Tensor& x, const Tensor& w, OptTensor residual, double eps)
   TORCH_CHECK_VALUE(std::isfinite(eps) && eps >= 0, "eps must be finite and not negative, got ", eps);
 }
 
-Tensor rows_of(const Tensor& t) { return t.contiguous().view({t.numel() / t.size(-1), t.size(-1)}); }
-
-// {y, h or undefined, rstd}, shaped like x
-std::vector<Tensor> rms_rows(const Tensor& x, const Tensor& w, OptTensor residual, double eps, bool need) {
-  auto r = rms_fwd(rows_of(x), w.contiguous(), given(residual) ? std::optional<Tensor>(rows_of(*residual)) : std::nullopt, eps, need);
-  r[0] = r[0].view(x.sizes());
-  if (given(residual)) r[1] = r[1].view(x.sizes());
-  return r;
-}
+OptTensor no_tensor = std::nullopt;
+std::optional<Tensor> dense(OptTensor t) { return given(t) ? std::optional<Tensor>(t->contiguous()) : std::nullopt; }
 
 struct RmsNormNode : public torch::autograd::Function<RmsNormNode> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, OptTensor residual, double eps) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto r = rms_rows(x, w, residual, eps, true);
+    auto r = rms_fwd(x.contiguous(), w.contiguous(), dense(residual), eps, true);
     ctx->set_materialize_grads(false);
     const bool sum = given(residual);
     ctx->saved_data["sum"] = sum;
@@ -443,17 +436,17 @@ struct RmsNormNode : public torch::autograd::Function<RmsNormNode> {
     const bool sum = ctx->saved_data["sum"].toBool();
     const Tensor dh = sum ? grads[1] : Tensor();
     if (!grads[0].defined()) return {dh, Tensor(), dh, Tensor()};
-    auto r = rms_bwd(rows_of(grads[0]), dh.defined() ? std::optional<Tensor>(rows_of(dh)) : std::nullopt, rows_of(s[0]), s[1].contiguous(), s[2]);
-    const Tensor dx = r[0].view(s[0].sizes());
-    return {dx, r[1], sum ? dx : Tensor(), Tensor()};
+    auto r = rms_bwd(grads[0].contiguous(), dh.defined() ? std::optional<Tensor>(dh.contiguous()) : std::nullopt, s[0].contiguous(),
+                     s[1].contiguous(), s[2]);
+    return {r[0], r[1], sum ? r[0] : Tensor(), Tensor()};
   }
 };
 
 Tensor rms_norm(const Tensor& x, const Tensor& w, double eps) {
-  rms_check(x, w, std::nullopt, eps);
+  rms_check(x, w, no_tensor, eps);
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w))) return RmsNormNode::apply(x, w, std::optional<Tensor>(), eps)[0];
   at::AutoDispatchBelowADInplaceOrView below;
-  return rms_rows(x, w, std::nullopt, eps, false)[0];
+  return rms_fwd(x.contiguous(), w.contiguous(), no_tensor, eps, false)[0];
 }
 
 std::tuple<Tensor, Tensor> rms_norm_residual(const Tensor& x, const Tensor& w, const Tensor& residual, double eps) {
@@ -463,7 +456,7 @@ std::tuple<Tensor, Tensor> rms_norm_residual(const Tensor& x, const Tensor& w, c
     return {r[0], r[1]};
   }
   at::AutoDispatchBelowADInplaceOrView below;
-  auto r = rms_rows(x, w, residual, eps, false);
+  auto r = rms_fwd(x.contiguous(), w.contiguous(), residual.contiguous(), eps, false);
   return {r[0], r[1]};
 }
 
@@ -473,11 +466,8 @@ std::vector<Tensor> rms_norm_int8(const Tensor& x, const Tensor& w, OptTensor re
   TORCH_CHECK(!at::GradMode::is_enabled() || !(wants_grad(x) || wants_grad(w) || (given(residual) && wants_grad(*residual))),
               "rms_norm_int8 has no gradient: call it under torch.no_grad()");
   at::AutoDispatchBelowADInplaceOrView below;
-  auto r = rms_fwd_int8(rows_of(x), w.contiguous(), given(residual) ? std::optional<Tensor>(rows_of(*residual)) : std::nullopt, eps);
-  r[0] = r[0].view(x.sizes());
-  r[1] = r[1].view(x.sizes().slice(0, x.dim() - 1));
-  if (given(residual)) r[2] = r[2].view(x.sizes());
-  else r.pop_back();
+  auto r = rms_fwd_int8(x.contiguous(), w.contiguous(), dense(residual), eps);
+  if (!given(residual)) r.pop_back();
   return r;
 }
 

@@ -353,6 +353,63 @@ def test_gradients_against_differences(ext_ops, dt):
 
 
 @pytest.mark.gpu
+def test_offsets_past_32_bits(ext_ops):
+    """One token over a cache of more than 2^31 values (4 GiB in bf16): keys and values in its last rows
+    and its first ones decide the output."""
+    heads, d = 8, 128
+    lk = (1 << 31) // (heads * d) + 777
+    cache = torch.zeros(1, lk, heads, d, dtype=torch.bfloat16, device=DEV)
+    gen = torch.Generator().manual_seed(4)
+    rows = torch.tensor([0, 5, lk - 300, lk - 2, lk - 1])
+    vals = torch.randn(len(rows), heads, d, generator=gen).to(torch.bfloat16)
+    cache[0, rows.to(DEV)] = vals.to(DEV)
+    q = (vals[-1:].float() * 3).to(torch.bfloat16).view(1, 1, heads, d).to(DEV)
+    out = attention(q, cache, cache, scale=0.1)
+    # the other lk - 5 keys have score 0 and value 0
+    s = 0.1 * torch.einsum('hd,jhd->hj', q[0, 0].cpu().double(), vals.double())
+    top = s.amax(1, keepdim=True).clamp(min=0)
+    p = (s - top).exp()
+    total = p.sum(1, keepdim=True) + (lk - len(rows)) * (-top).exp()
+    ref = torch.einsum('hj,jhd->hd', p / total, vals.double())
+    # P and the output rounded once each, 2^-8 relative; 1e-6 for the fp32 sum of lk terms
+    tol = 2.0 ** -7 * torch.einsum('hj,jhd->hd', p / total, vals.double().abs()) + 1e-6
+    assert ((out[0, 0].cpu().double() - ref).abs() <= tol).all()
+    last = attention(q, cache, cache, scale=0.1, lengths=torch.tensor([lk - 1], dtype=torch.int32, device=DEV))
+    assert (last.float().norm() < out.float().norm())
+
+
+@pytest.mark.gpu
+def test_one_derivative_only(ext_ops):
+    q, k, v, do = inputs(1, 40, 40, 1, 1, 32, torch.float32)
+    q.requires_grad_(True)
+    out = attention(q, k, v)
+    with pytest.raises(RuntimeError, match='second derivative'):
+        torch.autograd.grad(out, q, do, create_graph=True)
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(ext_ops):
+    """Calls on two streams share nothing: each gives what it gives alone."""
+    sets = [inputs(2, n, 900, 2, 2, 64, torch.bfloat16, seed=n) for n in (1, 130)]
+
+    def once(q, k, v, do):
+        q, k, v = (t.detach().requires_grad_(True) for t in (q, k, v))
+        out = attention(q, k, v)
+        return (out, *torch.autograd.grad(out, (q, k, v), do))
+    alone = [once(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = []
+    for _ in range(5):
+        for st, s in zip(streams, sets):
+            with torch.cuda.stream(st):
+                got.append(once(*s))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, alone[i % 2]))
+
+
+@pytest.mark.gpu
 def test_gpu_refusals(ext_ops):
     q, k, v, _ = inputs(1, 3, 6, 1, 1, 8, torch.float32)
     with pytest.raises(TypeError):

@@ -170,7 +170,13 @@ def test_layouts_and_unused_outputs(ext_ops, dt):
     full = torch.autograd.grad((y, h), (x, w), (dy, torch.zeros_like(dh)), retain_graph=True)
     only = torch.autograd.grad(y, (x, w), dy, retain_graph=True)
     assert all(torch.equal(a, b) for a, b in zip(full, only))
-    assert torch.equal(torch.autograd.grad(h, x, dh)[0], dh)
+    assert torch.equal(torch.autograd.grad(h, x, dh, retain_graph=True)[0], dh)
+    with pytest.raises(RuntimeError, match='second derivative'):
+        torch.autograd.grad(y, x, dy, create_graph=True)
+    one = rms_norm(x[0], w)                        # a single vector
+    assert one.shape == (96,) and torch.equal(one, rms_norm(x, w)[0])
+    q, s, none = rms_norm_int8(x[0].detach(), w.detach())
+    assert q.shape == (96,) and s.shape == () and none is None
 
 
 @pytest.mark.gpu
