@@ -402,20 +402,33 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   const int lane = threadIdx.x & 63;
   const int bh = (int)(w / R), row = (int)(w - (int64_t)bh * R);
   const int64_t p0 = (int64_t)bh * a.nsplit * R + row;
-  // lane s: the s-th range's maximum, sum and factor (at most 64 ranges)
+  // lane s: the s-th range's maximum, sum and factor (at most 64 ranges).  The first ranges' outputs are
+  // fetched beside them: the launch is a chain of memory latencies.
+  constexpr int PL = (DP + 63) / 64, PRE = 16;
   const bool mine = lane < a.nsplit;
   const float m = mine ? a.part_ml[2 * (p0 + (int64_t)lane * R)] : -INFINITY;
+  const float l = mine ? a.part_ml[2 * (p0 + (int64_t)lane * R) + 1] : 0.f;
+  float o[PL], pre[PRE][PL];
+#pragma unroll
+  for (int s = 0; s < PRE; ++s)
+#pragma unroll
+    for (int k = 0; k < PL; ++k)
+      pre[s][k] = s < a.nsplit && lane + 64 * k < DP ? a.part[(p0 + (int64_t)s * R) * DP + lane + 64 * k] : 0.f;
   float mt = m;
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) mt = fmaxf(mt, __shfl_xor(mt, x, 64));
   const float fs = __builtin_amdgcn_exp2f(m - (mt == -INFINITY ? 0.f : mt));
-  const float lt = wave_sum(mine ? a.part_ml[2 * (p0 + (int64_t)lane * R) + 1] * fs : 0.f);
-  constexpr int PL = (DP + 63) / 64;
-  float o[PL];
+  const float lt = wave_sum(mine ? l * fs : 0.f);
 #pragma unroll
   for (int k = 0; k < PL; ++k) o[k] = 0.f;
+#pragma unroll
+  for (int s = 0; s < PRE; ++s) {
+    const float f = __shfl(fs, s, 64);
+#pragma unroll
+    for (int k = 0; k < PL; ++k) o[k] += pre[s][k] * f;
+  }
 #pragma unroll 8
-  for (int s = 0; s < a.nsplit; ++s) {
+  for (int s = PRE; s < a.nsplit; ++s) {
     const float f = __shfl(fs, s, 64);
 #pragma unroll
     for (int k = 0; k < PL; ++k)
@@ -507,10 +520,12 @@ void fwd_dim(const AttnArgs& a, hipStream_t s) {
 void attn_fwd_plan(AttnArgs& a) {
   const int64_t R = (int64_t)a.G * a.Lq, heads = (int64_t)a.B * a.Hkv;
   // Enough workgroups for the 256 CUs: key ranges are split (and joined by a second launch) when the
-  // row tiles alone leave CUs idle; a range keeps at least 256 keys so the join stays small.
+  // row tiles alone leave CUs idle; a range keeps at least 256 keys (64 in fp32, whose products take 16
+  // times as long) so the join stays small.  Few rows: two workgroups a CU (32 caches of up to 16384
+  // keys: 304 us; with four or eight 306 and 308).
   const int64_t n = (R <= 32 ? 1 : (R + 127) / 128) * heads;
-  const int64_t want = R <= 32 ? 512 : 256;
-  const int64_t s = std::min<int64_t>(want / std::max<int64_t>(n, 1), (a.Lk + 255) / 256);
+  const int64_t want = R <= 32 ? 512 : 256, least = a.dtype == 2 ? 64 : 256;
+  const int64_t s = std::min<int64_t>(want / std::max<int64_t>(n, 1), (a.Lk + least - 1) / least);
   a.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(s, 64));
 }
 
