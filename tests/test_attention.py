@@ -284,6 +284,21 @@ def test_split_keys(ext_ops, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('dt', list(DTS))
+@pytest.mark.parametrize('lq,lk,g', [(3, 1500, 2), (40, 1500, 1), (1500, 40, 2), (900, 130, 3), (1300, 1, 1)])
+def test_split_walks_under_masks(ext_ops, dt, lq, lk, g):
+    """One side long, the other short: forward and backward split the long walk; masks and lengths on top."""
+    q, k, v, do = inputs(2, lq, lk, 1, g, 64, DTS[dt])
+    gen = torch.Generator().manual_seed(6)
+    full = (torch.rand(2, g, lq, lk, generator=gen) < 0.6).to(DEV)
+    lengths = torch.tensor([lk, (lk + 1) // 2], dtype=torch.int32, device=DEV)
+    check(q, k, v, do)
+    check(q, k, v, do, mask=full)
+    check(q, k, v, do, mask=full, lengths=lengths, causal=True, q_offset=lengths - lq)
+    check(q, k, v, do, mask=full[:, :1, :1], lengths=lengths)
+
+
+@pytest.mark.gpu
 def test_same_bits_again_and_other_stream(ext_ops):
     q, k, v, do = inputs(2, 333, 333, 2, 2, 64, torch.float16)
     q, k, v = (t.requires_grad_(True) for t in (q, k, v))
