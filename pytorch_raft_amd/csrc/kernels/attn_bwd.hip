@@ -10,6 +10,8 @@
 // kinds share a launch because a workgroup fills its CU (one wave per SIMD: 32 keys of dk and dv are
 // 128 accumulators): 12 x 2852 tokens make 276 workgroups of each kind for 256 CUs, and the dq ones
 // fill the second round of the others.
+// 12 x 2852 tokens, a head of 128, bf16: 240 us (745 TFLOP/s of the 7 products), 4 x 7040 x 4 heads 1560 us
+// (800); LDS fragment reads (32 KB a 32 x 32 block and wave) take as long as the matrix instructions.
 // In each kind the score tile lies so that it is the B operand of the gradient products as it is
 // (attn_common.h): dk / dv own keys as columns, dq owns rows as columns.
 //

@@ -4,6 +4,13 @@
 // of a key block are computed transposed, S^T = K Q^T, so that a lane holds one query's scores:
 // maximum and sum are register reductions plus one half-wave exchange, rescaling the output is one
 // multiply per register, and the probabilities are the B operand of O^T = V^T P^T as they lie.
+//
+// Four waves share the K and V tiles (64 keys; 32 in fp32), double-buffered by LDS-DMA, two workgroups a
+// CU.  bf16: 8 x 7040 tokens, 2 heads of 64: 250 us, 810 TFLOP/s -- the vector unit's work on the scores
+// (about 800 cycles a tile and wave, 512 of matrix instructions) bounds it; 4 x 7040, 4 heads of 128:
+// 420 us, 970 TFLOP/s, where LDS fragment reads and matrix instructions need the same time.  Forming the
+// next tile's scores ahead (295 us for the first), 3 or 4 waves a SIMD (302, 281) and 64 rows a wave (289)
+// measured slower.
 #include "attn_common.h"
 
 namespace attn_detail {
@@ -148,9 +155,8 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
 
   const int R = a.G * a.Lq;
   const int tiles = (R + C::BM - 1) / C::BM;
-  const int id = xcd_order(blockIdx.x, gridDim.x);
-  if (id >= tiles * a.nsplit * a.B * a.Hkv) return;
-  const int tile = tiles - 1 - id % tiles, split = id / tiles % a.nsplit, bh = id / tiles / a.nsplit;
+  int tile, split, bh;
+  if (!place(a, blockIdx.x, gridDim.x, tiles, a.nsplit, true, tile, split, bh)) return;
   const int b = bh / a.Hkv, hk = bh - b * a.Hkv;
   const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -209,6 +215,10 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
   };
   const uint32_t krow = TL::rows_base(raft_lds_addr(&kv[0][0][0]), lane), vcol = TL::cols_base(raft_lds_addr(&kv[0][1][0]), lane);
   const float c = a.scale_log2;
+  // Two waves share a SIMD: issue priority for one's score products parts their phases.  Heads of 128:
+  // 12 x 2852 tokens 85 us against 90, 4 x 7040 x 4 heads 420 / 430, causal 2 x 4096 x 16 142 / 151;
+  // smaller heads, bound by the vector unit, and fp32 gain nothing (198 / 194 with heads of 32).
+  constexpr bool FIRST = sizeof(T) == 2 && DP == 128;
   uint64_t next = 0;
   if (t0 < t1) {
     look(t0);
@@ -222,7 +232,9 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     if (t + 1 < t1) next = issue(t + 1, buf ^ 1);
     if (k0 >= wlim) continue;
     f32x16 s[NB];
+    if constexpr (FIRST) __builtin_amdgcn_s_setprio(1);
     st.scores(krow + buf * 2 * C::TILE, s);
+    if constexpr (FIRST) __builtin_amdgcn_s_setprio(0);
     if (MASK || k0 + BK > wmin)
       hide<NB, MASK>(s, lim - k0, hi, keys);
     st.raise(s, c);
@@ -249,7 +261,8 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
 
 // ---- few rows (R <= 32) over long keys: bound by reading K and V once.  The four waves of a
 // workgroup take different 32-key blocks of the workgroup's key range, each through LDS buffers of
-// its own (no barrier in the loop), and are joined in LDS at the end.
+// its own (no barrier in the loop), and are joined in LDS at the end.  32 items with caches of 8192 to
+// 16384 keys, 8 key heads of 128 in bf16: 1.63 GB in 304 us, 5.35 TB/s.
 template <typename T, int DP, int MASK>
 __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnArgs a) {
   using TL = Tile<T, DP>;

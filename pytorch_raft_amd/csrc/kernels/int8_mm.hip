@@ -5,6 +5,7 @@
 // Both operands lie with k innermost, which is what v_mfma_i32_32x32x32_i8 wants of A and B (16
 // consecutive k per lane).  w is the A operand and x the B operand, so a lane's accumulator holds 4
 // consecutive channels of one token: vector stores, one token scale per lane.
+// 8192 x 8192 x 4096 to bf16: 283 us, 1.94 POP/s (the library's int32 product without scales: 2.02).
 #include "common.h"
 #include "launchers.h"
 
@@ -248,7 +249,8 @@ __global__ __launch_bounds__(256, (BM * BN <= 128 * 128 ? 2 : 1)) void int8_tile
 
 // ---- few tokens (M <= 64): bound by reading w once.  A workgroup takes 16 channels, its 8 waves
 // split k in steps of 64 bytes (16x16x64: lane = channel row, 16 bytes at k (lane >> 4) * 16), all
-// straight from memory to registers; the waves' int32 sums meet in LDS.
+// straight from memory to registers; the waves' int32 sums meet in LDS.  5 x 4096 x 4096: 6 us (2.8 TB/s; one
+// workgroup a CU with 64 KB in flight, so a chain of two memory latencies and the launch).
 template <int MT, typename T>
 __global__ __launch_bounds__(512) void int8_few_kernel(Int8Args a) {
   __shared__ i32x4 sh[8][MT][64];

@@ -7,6 +7,8 @@
 // Bound by memory: a row is read once into registers (16-byte loads, EPT elements a thread), reduced
 // over the TPR threads that share it, and written.  TPR grows with the row (rule in rms_dispatch) so
 // that a thread holds 8 or 16 elements; groups walk the rows and keep the weight in registers.
+// 34224 x 256 bf16 with residual: forward 17 us, backward 17 us (4.1 TB/s each) and 4 us for dw; 16384 x 4096
+// to 8 bits with residual: 112 us (4.2 TB/s; a plain copy reaches 4.76).
 #include "common.h"
 #include "launchers.h"
 
