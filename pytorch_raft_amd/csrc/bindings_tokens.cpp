@@ -30,15 +30,17 @@ int dtype_code(const Tensor& t, const char* name) {
   return st == at::kBFloat16 ? 0 : (st == at::kHalf ? 1 : 2);
 }
 
-// (B, L, heads, D) whose rows the kernels can read in 16-byte pieces; anything else is copied once
-Tensor token_rows(const Tensor& t) {
+// (B, L, heads, D) whose rows the kernels can read in 16-byte pieces; anything else is copied once.
+// heads: that one tile of rows spans (the backward walks the query heads of a group in one).
+Tensor token_rows(const Tensor& t, int64_t heads = 1) {
   const int64_t es = t.element_size();
   bool ok = t.stride(3) == 1 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
   int64_t reach = 0;
   for (int d = 0; d < 3; ++d) {
     if (t.size(d) == 1) continue;
     ok = ok && t.stride(d) * es % 16 == 0 && t.stride(d) >= t.size(3);
-    if (d > 0) reach += t.stride(d) * es * std::min<int64_t>(t.size(d), 72);
+    if (d == 1) reach += t.stride(d) * es * std::min<int64_t>(t.size(d), 72);
+    if (d == 2) reach += t.stride(d) * es * (heads - 1);
   }
   ok = ok && reach < (int64_t(1) << 30);  // a tile's rows lie within a descriptor's 32-bit offsets
   // (.contiguous() alone would keep a dense tensor that starts off 16 bytes)
@@ -151,7 +153,8 @@ std::vector<Tensor> attn_bwd(const Tensor& dout0, const Tensor& q0, const Tensor
   c10::DeviceGuard g(q0.device());
   TORCH_CHECK(dout0.device() == q0.device() && dout0.scalar_type() == q0.scalar_type() && dout0.sizes() == q0.sizes(),
               "dout must match q");
-  const Tensor q = token_rows(q0), k = token_rows(k0), v = token_rows(v0), dout = token_rows(dout0);
+  const int64_t group = k0.size(2) > 0 ? std::max<int64_t>(q0.size(2) / k0.size(2), 1) : 1;
+  const Tensor q = token_rows(q0, group), k = token_rows(k0), v = token_rows(v0), dout = token_rows(dout0, group);
   AttnArgs a = attn_args(q, k, v, scale, causal, mask, lengths, q_offset);
   const int64_t R = (int64_t)a.G * a.Lq;
   TORCH_CHECK(out.device() == q.device() && out.scalar_type() == q.scalar_type() && out.sizes() == q.sizes() && out.is_contiguous(),

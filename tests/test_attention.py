@@ -394,6 +394,30 @@ def test_offsets_past_32_bits(ext_ops):
 
 
 @pytest.mark.gpu
+def test_query_heads_far_apart(ext_ops):
+    """160 heads of one group, 14 MB from each other: the last lies past 2^31 bytes of the first."""
+    q, k, v, do = inputs(1, 5, 65, 1, 160, 8, torch.bfloat16)
+    far = torch.zeros(160, 7_000_000, dtype=q.dtype, device=DEV)
+    far[:, :40] = q[0].transpose(0, 1).reshape(160, 40)
+    check(far[:, :40].unflatten(1, (5, 8)).transpose(0, 1)[None], k, v, do)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('lq', [1, 40])
+def test_long_head_major_cache_is_not_copied(ext_ops, lq):
+    n = 1 << 18
+    cache = torch.randn(1, 20, n, 128, device=DEV, dtype=torch.bfloat16).transpose(1, 2)  # 1.3 GB
+    q = torch.randn(1, lq, 20, 128, device=DEV, dtype=torch.bfloat16)
+    lengths = torch.tensor([n - 3], dtype=torch.int32, device=DEV)
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = attention(q, cache, cache, lengths=lengths, impl='hip')
+    assert torch.cuda.max_memory_allocated() - before < 1 << 29
+    # the same values in the other order of memory give the same bits
+    assert torch.equal(out, attention(q, cache.contiguous(), cache.contiguous(), lengths=lengths, impl='hip'))
+
+
+@pytest.mark.gpu
 def test_one_derivative_only(ext_ops):
     q, k, v, do = inputs(1, 40, 40, 1, 1, 32, torch.float32)
     q.requires_grad_(True)
