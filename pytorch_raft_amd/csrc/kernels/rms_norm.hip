@@ -136,14 +136,15 @@ __global__ __launch_bounds__((Rows<T, TPR, EPT>::NT)) void rms_fwd_kernel(RmsArg
 #pragma unroll
       for (int i = 0; i < EPT; ++i) top = max(top, __float_as_uint(h[i]) & 0x7fffffffu);
       const float m = __uint_as_float(group_max<TPR>(top, reinterpret_cast<uint32_t*>(sh)));
-      const float inv = m == 0.f ? 0.f : 127.f / m;
+      // (127 / m passes fp32's range under m = 2^-121: such rows are raised by 2^64 first, exactly)
+      const float up = m < 0x1p-100f ? 0x1p64f : 1.f, inv = m == 0.f ? 0.f : 127.f / (m * up);
 #pragma unroll
       for (int v = 0; v < R::NV; ++v) {
         const int e = R::at(v);
         struct { int8_t b[R::N]; } q;
 #pragma unroll
         for (int i = 0; i < R::N; ++i)
-          q.b[i] = (int8_t)(int)rintf(fminf(fmaxf(h[v * R::N + i] * inv, -127.f), 127.f));
+          q.b[i] = (int8_t)(int)rintf(fminf(fmaxf(h[v * R::N + i] * up * inv, -127.f), 127.f));
         int8_t* p = reinterpret_cast<int8_t*>(a.y) + row * a.C + e;
         if (C - e >= R::N) __builtin_memcpy(p, &q, R::N);
         else

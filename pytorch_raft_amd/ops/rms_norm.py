@@ -36,7 +36,9 @@ def torch_rms_norm(x, weight, residual=None, eps=1e-6):
 def torch_rms_norm_int8(x, weight, residual=None, eps=1e-6):
     y, h = _torch_norm(x, weight, residual, eps)
     top = y.abs().amax(-1, keepdim=True)
-    q = torch.round(y * torch.where(top == 0, torch.zeros_like(top), 127 / top)).clamp(-127, 127)
+    # (127 / top passes fp32's range for rows under 2^-121)
+    up = torch.where(top < 2. ** -100, 2. ** 64, 1.).to(top.dtype)
+    q = torch.round(y * up * torch.where(top == 0, torch.zeros_like(top), 127 / (top * up))).clamp(-127, 127)
     return q.nan_to_num(0.).to(torch.int8), (top / 127).squeeze(-1), None if residual is None else h
 
 

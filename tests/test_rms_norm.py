@@ -108,6 +108,26 @@ def test_plain_8_bit():
     assert ((q.float() * s[:, None] - y).abs() <= 0.5001 * s[:, None]).all()
 
 
+def tiny_rows(dev, impl):
+    """Rows whose largest value is under 2^-121, where 127 over it passes fp32's range: a power of two on
+    the weight changes no quotient (y stays a normal number where it is compared)."""
+    x, _, weight, _, _ = inputs(6, 100, torch.float32, dev=dev)
+    x[0, :50] = 0
+    weight = weight.sign() * weight.abs().clamp(0.5, 2)
+    q, scale, _ = rms_norm_int8(x, weight, impl=impl)
+    small, tiny, _ = rms_norm_int8(x, weight * 2.0 ** -123, impl=impl)
+    # a value under 2^-126 may lose bits of its own: at most half a step of 2^-149 against a step of
+    # max / 127 > 2^-131, so a quotient moves by less than 2^-18 and q by one where it lay that near a tie
+    d = (small.int() - q.int()).abs()
+    assert d.max() <= 1 and (d != 0).sum() <= 2
+    assert (small[0, :50] == 0).all() and small.abs().amax(-1).eq(127).all()
+    assert ((tiny.double() * 2.0 ** 123 - scale.double()).abs() <= 2.0 ** -17 * scale.double()).all()
+
+
+def test_plain_8_bit_of_tiny_rows():
+    tiny_rows('cpu', 'torch')
+
+
 def test_refusals():
     x, r, w, _, _ = inputs(4, 16, torch.float32, dev='cpu')
     for args, kw in (((x, w[:8]), {}), ((x, w), {'residual': r[:3]}), ((x, w), {'residual': r.half()}),
@@ -191,6 +211,11 @@ def test_special_rows(ext_ops):
     q, s, _ = rms_norm_int8(x, w)
     assert s[1] == 0 and (q[1] == 0).all() and torch.isnan(s[3]) and torch.isnan(s[4])
     check8(x[[0, 1, 2, 5]], None, w)
+
+
+@pytest.mark.gpu
+def test_8_bit_of_tiny_rows(ext_ops):
+    tiny_rows(DEV, 'hip')
 
 
 @pytest.mark.gpu
