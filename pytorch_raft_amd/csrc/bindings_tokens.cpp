@@ -72,8 +72,10 @@ AttnArgs attn_args(const Tensor& q, const Tensor& k, const Tensor& v, double sca
   TORCH_CHECK(D >= 8 && D <= 128 && D % 8 == 0, "head size must be a multiple of 8 up to 128, got ", D);
   TORCH_CHECK(std::isfinite(scale) && scale > 0, "scale must be positive and finite");
   const int64_t big = int64_t(1) << 26;
-  TORCH_CHECK(B * H * std::max<int64_t>(Lq, 1) < big && B * k.size(2) * std::max<int64_t>(Lk, 1) < big * 16 && Lk < big * 16,
-              "attention: too many rows for one call");
+  // (grids: less than 2^24 workgroups of 256)
+  TORCH_CHECK(B * H * std::max<int64_t>(Lq, 1) < big && B * k.size(2) * std::max<int64_t>(Lk, 1) < big * 16 && Lk < big * 16 &&
+                  B * k.size(2) < big / 16,
+              "attention: too many rows or heads for one call");
   AttnArgs a = {};
   a.dtype = dtype_code(q, "q");
   a.B = (int)B;

@@ -461,3 +461,16 @@ def test_gpu_refusals(ext_ops):
         ext_ops.attn_fwd(q, k, v[:, :5], 1.0, False, None, None, None, False)
     with pytest.raises(RuntimeError):
         ext_ops.attn_fwd(q, k, v, -1.0, False, None, None, None, False)
+
+
+@pytest.mark.gpu
+def test_most_heads_of_a_call(ext_ops):
+    many = torch.zeros(1 << 22, 1, 1, 8, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(RuntimeError):
+        attention(many, many, many)
+    many[-1] = 2
+    q = many[1:].requires_grad_(True)
+    out = attention(q, q, q)
+    assert out[:-1].count_nonzero() == 0 and (out[-1] == 2).all()
+    out.backward(torch.ones_like(out))
+    assert (q.grad == 1).all()  # one key: dv = dout, no gradient through the scores
