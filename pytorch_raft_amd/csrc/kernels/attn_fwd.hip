@@ -462,46 +462,48 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 }
 
 // A wave per 64 rows x 64 keys: a lane gathers its row's 64 bytes into a word; ballots over the words
-// turn the square for the keys' words.
+// turn the square for the keys' words.  (A grid of bounded size walks them: a broadcast mask has no
+// memory of its own that would bound them.)
 __global__ __launch_bounds__(256) void attn_pack_kernel(AttnArgs a) {
   const int R = a.G * a.Lq, nrt = (R + 63) / 64, nkt = (a.Lk + 63) / 64, nh = a.m_sh ? a.Hkv : 1, nb = a.m_sb ? a.B : 1;
-  const int64_t w = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (w >= (int64_t)nb * nh * nrt * nkt) return;
-  const int lane = threadIdx.x & 63;
-  const int kt = (int)(w % nkt), rt = (int)(w / nkt % nrt), hk = (int)(w / nkt / nrt % nh), b = (int)(w / nkt / nrt / nh);
-  const int row = rt * 64 + lane, rc = min(row, R - 1), qi = rc / a.G, h = hk * a.G + rc - qi * a.G;
-  const uint8_t* p = a.mask + b * a.m_sb + h * a.m_sh + (int64_t)qi * a.m_sq + (int64_t)kt * 64 * a.m_sk;
-  const int n = min(64, a.Lk - kt * 64);
-  uint64_t mine = 0;
-  if (a.m_sk == 1 && n == 64) {
+  const int64_t words = (int64_t)nb * nh * nrt * nkt;
+  for (int64_t w = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); w < words; w += (int64_t)gridDim.x * 4) {
+    const int lane = threadIdx.x & 63;
+    const int kt = (int)(w % nkt), rt = (int)(w / nkt % nrt), hk = (int)(w / nkt / nrt % nh), b = (int)(w / nkt / nrt / nh);
+    const int row = rt * 64 + lane, rc = min(row, R - 1), qi = rc / a.G, h = hk * a.G + rc - qi * a.G;
+    const uint8_t* p = a.mask + b * a.m_sb + h * a.m_sh + (int64_t)qi * a.m_sq + (int64_t)kt * 64 * a.m_sk;
+    const int n = min(64, a.Lk - kt * 64);
+    uint64_t mine = 0;
+    if (a.m_sk == 1 && n == 64) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      uint4 v;
-      __builtin_memcpy(&v, p + 16 * c, 16);  // any alignment
-      const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+      for (int c = 0; c < 4; ++c) {
+        uint4 v;
+        __builtin_memcpy(&v, p + 16 * c, 16);  // any alignment
+        const uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // bit 0 of each byte = any of its bits, then the four bits side by side
-        uint32_t y = x[i] | x[i] >> 4;
-        y |= y >> 2;
-        y = (y | y >> 1) & 0x01010101u;
-        mine |= (uint64_t)(y * 0x10204080u >> 28) << (16 * c + 4 * i);
+        for (int i = 0; i < 4; ++i) {
+          // bit 0 of each byte = any of its bits, then the four bits side by side
+          uint32_t y = x[i] | x[i] >> 4;
+          y |= y >> 2;
+          y = (y | y >> 1) & 0x01010101u;
+          mine |= (uint64_t)(y * 0x10204080u >> 28) << (16 * c + 4 * i);
+        }
       }
+    } else {
+      for (int k = 0; k < n; ++k) mine |= (uint64_t)(p[(int64_t)k * a.m_sk] != 0) << k;
     }
-  } else {
-    for (int k = 0; k < n; ++k) mine |= (uint64_t)(p[(int64_t)k * a.m_sk] != 0) << k;
-  }
-  if (row >= R) mine = 0;
-  const int64_t head = (int64_t)b * nh + hk;
-  if (row < R) a.row_bits[(head * R + row) * nkt + kt] = mine;
-  if (a.key_bits) {
-    uint64_t col = 0;
+    if (row >= R) mine = 0;
+    const int64_t head = (int64_t)b * nh + hk;
+    if (row < R) a.row_bits[(head * R + row) * nkt + kt] = mine;
+    if (a.key_bits) {
+      uint64_t col = 0;
 #pragma unroll
-    for (int k = 0; k < 64; ++k) {
-      const uint64_t bits = __ballot(mine >> k & 1);
-      if (lane == k) col = bits;
+      for (int k = 0; k < 64; ++k) {
+        const uint64_t bits = __ballot(mine >> k & 1);
+        if (lane == k) col = bits;
+      }
+      if (lane < n) a.key_bits[(head * a.Lk + kt * 64 + lane) * nrt + rt] = col;
     }
-    if (lane < n) a.key_bits[(head * a.Lk + kt * 64 + lane) * nrt + rt] = col;
   }
 }
 
@@ -550,7 +552,7 @@ int64_t attn_bit_words(const AttnArgs& a, bool keys) {
 
 void launch_attn_pack(const AttnArgs& a, hipStream_t s) {
   const int64_t R = (int64_t)a.G * a.Lq, heads = (int64_t)(a.m_sb ? a.B : 1) * (a.m_sh ? a.Hkv : 1);
-  attn_detail::attn_pack_kernel<<<raft_cdiv(heads * ((R + 63) / 64) * ((a.Lk + 63) / 64), 4), 256, 0, s>>>(a);
+  attn_detail::attn_pack_kernel<<<(unsigned)std::min<int64_t>((heads * ((R + 63) / 64) * ((a.Lk + 63) / 64) + 3) / 4, 2048), 256, 0, s>>>(a);
 }
 
 void launch_attn_fwd(const AttnArgs& a, hipStream_t s) {

@@ -290,12 +290,13 @@ __global__ __launch_bounds__(512) void int8_few_kernel(Int8Args a) {
 
 // x and w with rows of kp (a multiple of 16) bytes, zeros from K on, in `to` (16 bytes a thread)
 __global__ __launch_bounds__(256) void int8_pack_kernel(const int8_t* x, const int8_t* w, int8_t* to, int64_t M, int64_t N, int K, int kp) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = i / (kp / 16);
-  const int k = (int)(i - row * (kp / 16)) * 16;
-  if (row >= M + N) return;
-  const i32x4 v = load16(row < M ? x + row * K : w + (row - M) * K, k, K);
-  *reinterpret_cast<i32x4*>(to + row * kp + k) = v;
+  const int64_t chunks = (M + N) * (kp / 16);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / (kp / 16);
+    const int k = (int)(i - row * (kp / 16)) * 16;
+    const i32x4 v = load16(row < M ? x + row * K : w + (row - M) * K, k, K);
+    *reinterpret_cast<i32x4*>(to + row * kp + k) = v;
+  }
 }
 
 bool on16(const Int8Args& a) { return a.K % 16 == 0 && (((uintptr_t)a.x | (uintptr_t)a.w) & 15) == 0; }
@@ -324,7 +325,7 @@ void mm(const Int8Args& a, hipStream_t s) {
       p.K = (a.K + 15) / 16 * 16;
       p.x = a.packed;
       p.w = a.packed + (int64_t)a.M * p.K;
-      int8_pack_kernel<<<raft_cdiv(((int64_t)a.M + a.N) * (p.K / 16), 256), 256, 0, s>>>(a.x, a.w, a.packed, a.M, a.N, a.K, p.K);
+      int8_pack_kernel<<<(unsigned)std::min<int64_t>((((int64_t)a.M + a.N) * (p.K / 16) + 255) / 256, 2048), 256, 0, s>>>(a.x, a.w, a.packed, a.M, a.N, a.K, p.K);
     }
     int8_tile_kernel<256, 256, 2, true, T><<<raft_cdiv((int64_t)raft_cdiv(a.M, 256) * raft_cdiv(a.N, 256), 8) * 8, 256, 0, s>>>(p);
   } else if ((int64_t)raft_cdiv(a.M, 128) * raft_cdiv(a.N, 128) >= 256) {
