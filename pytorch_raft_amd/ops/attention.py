@@ -18,8 +18,8 @@ A query that sees no key gets zeros, and zero gradients.  bf16, fp16 and fp32; s
 accumulators are fp32, the probabilities are rounded to the inputs' type for their product with v.
 Differentiable in q, k and v (the backward recomputes the probabilities from a saved log-sum-exp; the
 same inputs give the same bits).  Head sizes up to 128 (others than multiples of 8 are padded by a
-copy).  A call takes less than 2^22 pairs of item and key head and less than 2^26 rows (B * H * Lq).  Calls with at most 32 rows (H / Hkv * Lq), e.g. single tokens over a cache, run a kernel that
-splits the keys.
+copy); less than 2^22 pairs of item and key head and less than 2^26 rows (B * H * Lq) a call.  Calls with
+at most 32 rows (H / Hkv * Lq), e.g. single tokens over a cache, run a kernel that splits the keys.
 
 The all-pairs correlation (ops/corr.py) is the same product of two feature maps without the softmax.
 """
