@@ -394,6 +394,19 @@ def test_offsets_past_32_bits(ext_ops):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('dt', list(DTS))
+@pytest.mark.parametrize('causal', [False, True])
+@pytest.mark.parametrize('first,last', [(0, 130), (70, 290), (64, 256), (250, 400), (0, 400)])
+def test_padding_masks_of_whole_tiles(ext_ops, dt, causal, first, last):
+    """Keys first .. last - 1 of the first item hidden (the second item sees all), whatever they hold."""
+    q, k, v, do = inputs(2, 150, 400, 2, 1, 64, DTS[dt])
+    mask = torch.ones(2, 1, 1, 400, dtype=torch.bool, device=DEV)
+    mask[0, ..., first:last] = False
+    k[0, first:last], v[0, first:last] = float('nan'), float('inf')
+    check(q, k, v, do, mask=mask, causal=causal, lengths=torch.tensor([400, 390], dtype=torch.int32, device=DEV))
+
+
+@pytest.mark.gpu
 def test_query_heads_far_apart(ext_ops):
     """160 heads of one group, 14 MB from each other: the last lies past 2^31 bytes of the first."""
     q, k, v, do = inputs(1, 5, 65, 1, 160, 8, torch.bfloat16)
