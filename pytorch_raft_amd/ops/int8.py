@@ -22,7 +22,9 @@ def quantize_weight(weight):
         raise ValueError('weight must be a floating (N, K) tensor, got %s %s' % (weight.dtype, tuple(weight.shape)))
     w = weight.detach().float()
     top = w.abs().amax(1, keepdim=True) if w.shape[1] else w.new_zeros(w.shape[0], 1)
-    q = torch.round(w * torch.where(top == 0, torch.zeros_like(top), 127 / top)).clamp_(-127, 127)
+    # (127 / top passes fp32's range for rows under 2^-121: they are raised by 2^64 first, exactly)
+    up = torch.where(top < 2. ** -100, 2. ** 64, 1.).to(top.dtype)
+    q = torch.round(w * up * torch.where(top == 0, torch.zeros_like(top), 127 / (top * up))).clamp_(-127, 127)
     return q.to(torch.int8), (top / 127).squeeze(1)
 
 
