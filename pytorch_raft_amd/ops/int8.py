@@ -17,7 +17,7 @@ _CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
 def quantize_weight(weight):
-    """(N, K) floating weight -> (int8 (N, K), fp32 scale (N,)), symmetric per output channel; once, not per call."""
+    """(N, K) floating weight -> (int8 (N, K), fp32 scale (N,)), contiguous, symmetric per output channel; once, not per call."""
     if weight.dim() != 2 or not weight.is_floating_point():
         raise ValueError('weight must be a floating (N, K) tensor, got %s %s' % (weight.dtype, tuple(weight.shape)))
     w = weight.detach().float()
@@ -25,7 +25,8 @@ def quantize_weight(weight):
     # (127 / top passes fp32's range for rows under 2^-121: they are raised by 2^64 first, exactly)
     up = torch.where(top < 2. ** -100, 2. ** 64, 1.).to(top.dtype)
     q = torch.round(w * up * torch.where(top == 0, torch.zeros_like(top), 127 / (top * up))).clamp_(-127, 127)
-    return q.to(torch.int8), (top / 127).squeeze(1)
+    # (rows of k one after the other, also for a transposed weight: int8_linear would copy it every call)
+    return q.to(torch.int8).contiguous(), (top / 127).reshape(-1)
 
 
 def torch_int8_linear(x, x_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16):

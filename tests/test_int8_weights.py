@@ -16,3 +16,15 @@ def test_tiny_rows():
         assert torch.equal(q[2], want) and not q[1].any() and s[1] == 0
         # the scale is rounded to fp32 once, under 2^-126 to a multiple of 2^-149
         assert abs(s[0].double() - 2.0 ** e / 127) <= max(2.0 ** -24 * 2.0 ** e / 127, 2.0 ** -150)
+
+
+def test_layout():
+    """The product reads rows of k: whatever the layout of the weight, no call copies the result again."""
+    w = torch.randn(32, 48, generator=torch.Generator().manual_seed(0))
+    q, s = quantize_weight(w)
+    wide = torch.zeros(32, 96)
+    wide[:, ::2] = w
+    for other in (w.t().contiguous().t(), wide[:, ::2], w.t().contiguous().double().t()):
+        q2, s2 = quantize_weight(other)
+        assert q2.is_contiguous() and s2.is_contiguous()
+        assert torch.equal(q2, q) and torch.equal(s2, s)
