@@ -104,6 +104,8 @@ __global__ __launch_bounds__(256) void attn_prep_kernel(AttnArgs a) {
       }
     }
     s = raft_row16_sum(s);
+    // a row that sees no key has no part in the gradients, whatever dout holds there
+    if (w < nrow && a.lse[w] == INFINITY) s = n = 0.f;
     if (w < nrow && sub == 0) a.delta[w] = s;
     if constexpr (F16) {
       n = raft_row16_sum(n);
@@ -239,14 +241,27 @@ __device__ __forceinline__ void dkv_body(const AttnArgs& a, int bid, int grid, u
     }
   };
   offsets(0, 0);
+  // Rows that see no key come as zeros: their q and dout may hold anything, and P = 0 times an infinity is
+  // NaN.  Without a mask those are the first ones under causal; under masks their lse says so (+inf), looked
+  // up a tile ahead and turned into bits by a ballot.
+  const int first = a.causal ? max(0, -off) * a.G : 0;
+  float ahead = INFINITY;
+  auto look = [&](int t) {
+    if constexpr (MASK != 0) {
+      const int r = t * BT + (lane & (BT - 1));
+      ahead = r < R ? lse[r] : INFINITY;
+    }
+  };
   auto issue = [&](int t, uint32_t buf, int sbuf) {
     const int r0 = t * BT, q0 = r0 / a.G;
+    const uint64_t rows = MASK != 0 ? __ballot(ahead != INFINITY) >> L::row_of(tid, 0) : 0;
     const rsrc_t rq = rsrc_of(qb + (int64_t)q0 * a.q_sl * TL::ES, 0x7fffffffu);
     const rsrc_t rd = rsrc_of(db + (int64_t)q0 * a.d_sl * TL::ES, 0x7fffffffu);
     if (!even) offsets(r0, q0);
 #pragma unroll
     for (int j = 0; j < L::PER; ++j) {
-      const bool ok = r0 + L::row_of(tid, j) < R;
+      const int r = r0 + L::row_of(tid, j);
+      const bool ok = MASK != 0 ? rows >> j * (256 / TL::NC) & 1 : r >= first && r < R;
       raft_dma16(rq, lds + buf + j * 4096, ok ? oq[j] : kOob);
       raft_dma16(rd, lds + buf + TILE + j * 4096, ok ? od[j] : kOob);
     }
@@ -255,6 +270,7 @@ __device__ __forceinline__ void dkv_body(const AttnArgs& a, int bid, int grid, u
       // rows past the last: P = 0
       stat[sbuf + tid] = tid < BT ? (r < R ? (F16 ? kP16 : 0.f) - lse[r] : -INFINITY) : (r < R ? dl[r] * ds_mul : 0.f);
     }
+    if (t + 1 < t1) look(t + 1);
   };
 
   // A tile of two 32-row blocks (16-bit types): scores and dP of both, exponentials of the first beside
@@ -300,7 +316,7 @@ __device__ __forceinline__ void dkv_body(const AttnArgs& a, int bid, int grid, u
       }
     }
     if constexpr (decltype(edge)::value) {
-      // a hidden place adds nothing, whatever dout holds (a hidden key's column is dropped at the end)
+      // a hidden place has no P and no dS (a hidden key's column is dropped at the end)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int row = row0 + (r >> 2) * 8 + hi * 4 + (r & 3);
@@ -365,6 +381,7 @@ __device__ __forceinline__ void dkv_body(const AttnArgs& a, int bid, int grid, u
     s0 = s1, s1 = s2, s2 = y;
   };
   if (t0 < t1) {
+    look(t0);
     issue(t0, b0, s0);
     if (t0 + 1 < t1) issue(t0 + 1, b1, s1);
     raft_wait_vmcnt<0>();

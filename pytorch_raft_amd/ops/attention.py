@@ -14,7 +14,9 @@ projection.
   mask that is the same for all queries and heads (a padding mask (B, 1, 1, Lk)) may hold anything; under a mask that
   differs between queries, and under ``causal``, keys and values must be finite.
 
-A query that sees no key gets zeros, and zero gradients.  bf16, fp16 and fp32; sums, maxima and
+A query that sees no key gets zeros, and zero gradients, and adds nothing to those of keys and values: it
+and its output's gradient may hold anything.  Where a query sees a key, an infinity or NaN in it, in what
+it sees or in its output's gradient may reach all gradients of its head.  bf16, fp16 and fp32; sums, maxima and
 accumulators are fp32, the probabilities are rounded to the inputs' type for their product with v.
 Differentiable in q, k and v (the backward recomputes the probabilities from a saved log-sum-exp; the
 same inputs give the same bits).  Head sizes up to 128 (others than multiples of 8 are padded by a
@@ -50,11 +52,12 @@ def torch_attention(q, k, v, scale=None, causal=False, mask=None, lengths=None, 
     used = see.any(1).any(1)[:, :, None, None]
     k = torch.where(used, k, torch.zeros_like(k)).repeat_interleave(h // hkv, 2)
     v = torch.where(used, v, torch.zeros_like(v)).repeat_interleave(h // hkv, 2)
+    # and so may queries that see no key, and their gradients
+    none = ~see.any(-1, keepdim=True)
+    q = q.masked_fill(none.transpose(1, 2), 0.)
     s = torch.matmul(q.transpose(1, 2).contiguous(), k.permute(0, 2, 3, 1).contiguous()) * scale
-    some = see.any(-1, keepdim=True)
-    s = s.masked_fill(~see, float('-inf')).masked_fill(~some, 0.)
-    p = torch.softmax(s, -1).masked_fill(~some, 0.) if lk else s
-    return torch.matmul(p, v.transpose(1, 2).contiguous()).transpose(1, 2)
+    p = torch.softmax(s.masked_fill(~see, float('-inf')).masked_fill(none, 0.), -1) if lk else s
+    return torch.matmul(p, v.transpose(1, 2).contiguous()).transpose(1, 2).masked_fill(none.transpose(1, 2), 0.)
 
 
 def _check(q, k, v, scale, mask, lengths, q_offset):

@@ -1,0 +1,70 @@
+"""Token attention (ops/attention.py) at the edges of what its documentation allows: queries that see no
+key and hold anything, single keys, scales at the ends of fp32's range, forward-mode derivatives, and
+the accuracy that the backward's row sums owe to the unrounded output.
+"""
+import pytest
+import torch
+
+from pytorch_raft_amd.ops.attention import attention
+from test_attention import DEV, DTS, close, formula, inputs
+
+
+def unseen_cases(dev):
+    """(mask, lengths, causal, q_offset, which queries (B, H, Lq) see a key) over 2 items, 2 x 2 heads,
+    150 queries and 170 keys: rows hidden by a mask for each row, causal rows before the first key (with
+    and without lengths), and causal rows whose keys up to their own position are all padding."""
+    b, h, lq, lk = 2, 4, 150, 170
+    gen = torch.Generator().manual_seed(8)
+    full = torch.rand(b, h, lq, lk, generator=gen) < 0.6
+    full[0, :, 17] = False
+    full[1, 2, 64:131] = False          # more than a whole tile of rows, one head
+    full[1, :, 149] = False
+    pos = torch.arange(lq)
+    before = torch.tensor([-70, -1], dtype=torch.int32)
+    lengths = torch.tensor([170, 3], dtype=torch.int32)
+    left = torch.ones(b, 1, 1, lk, dtype=torch.bool)
+    left[0, ..., :75] = False
+    left[1, ..., :1] = False
+    at = torch.tensor([0, 0], dtype=torch.int32)
+    all_heads = lambda t: t[:, None].expand(b, h, lq)  # noqa: E731
+    return [
+        (full.to(dev), None, False, None, full.any(-1)),
+        (None, None, True, before.to(dev), all_heads(pos + before[:, None] >= 0)),
+        (None, lengths.to(dev), True, before.to(dev), all_heads(pos + before[:, None] >= 0)),
+        (left.to(dev), None, True, at.to(dev), all_heads(pos >= torch.tensor([75, 1])[:, None])),
+        (full.to(dev), lengths.to(dev), True, at.to(dev),
+         (full & (torch.arange(lk) <= pos[:, None]) & (torch.arange(lk) < lengths[:, None, None, None])).any(-1)),
+    ]
+
+
+def check_unseen(dt, dev, case):
+    mask, lengths, causal, q_offset, seen = unseen_cases(dev)[case]
+    q, k, v, do = inputs(2, 150, 170, 2, 2, 40, dt, dev=dev)
+    kw = dict(mask=mask, lengths=lengths, causal=causal, q_offset=q_offset)
+    hidden = ~seen.transpose(1, 2).to(dev)                      # (B, Lq, H)
+    assert hidden.any() and not hidden.all()
+    q0, do0 = (t.masked_fill(hidden[..., None], 0) for t in (q, do))
+    res = formula(q0, k, v, do0, **kw)
+    for bad_q, bad_do in ((float('nan'), float('inf')), (float('-inf'), float('nan')), (float('inf'), torch.finfo(dt).max)):
+        q1 = q.masked_fill(hidden[..., None], bad_q).requires_grad_(True)
+        do1 = do.masked_fill(hidden[..., None], bad_do)
+        k1, v1 = (t.detach().requires_grad_(True) for t in (k, v))
+        out = attention(q1, k1, v1, **kw)
+        assert (out[hidden] == 0).all()
+        close(out, res, 'out')
+        grads = torch.autograd.grad(out, (q1, k1, v1), do1)
+        assert (grads[0][hidden] == 0).all()
+        for n, t in zip(('dq', 'dk', 'dv'), grads):
+            close(t, res, n)
+
+
+@pytest.mark.parametrize('case', range(5))
+def test_plain_form_queries_without_keys(case):
+    check_unseen(torch.float32, 'cpu', case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dt', list(DTS))
+@pytest.mark.parametrize('case', range(5))
+def test_queries_without_keys(ext_ops, dt, case):
+    check_unseen(DTS[dt], DEV, case)
