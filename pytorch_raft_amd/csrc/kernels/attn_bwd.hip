@@ -55,7 +55,7 @@ __device__ __forceinline__ float ds_scale(const AttnArgs& a) {
       m1 = max(m1, (uint32_t)__shfl_xor((int)m1, o, 64));
     }
     const float bound = 2.f * sqrtf(__uint_as_float(m0)) * sqrtf(__uint_as_float(m1));
-    if (!(bound > 0.f) || !(bound < INFINITY)) return 1.f;
+    if (!(bound > 0.f)) return 1.f;  // (finite: squares of fp16 values)
     const int e = 14 - (int)ceilf(log2f(bound));
     return ldexpf(1.f, max(-100, min(100, e)));
   } else {
@@ -65,8 +65,10 @@ __device__ __forceinline__ float ds_scale(const AttnArgs& a) {
 
 // delta of every row, from the output as a pair of 16-bit values (rounded value and what the rounding
 // took away): where one key takes nearly all of a row, dP - delta cancels, and a delta from the rounded
-// output alone left errors in dq and dk of up to 2.5 times the rounding of the result.  fp16: also the largest squared 2-norm of a dout row and of a v row that this
-// block met, as float bits (ordered like the floats, NaN above all).  16 lanes of 8 channels a row.
+// output alone left errors in dq and dk of up to 2.5 times the rounding of the result.  fp16: also the
+// largest squared 2-norm of a dout row and of a v row that this block met, as float bits (ordered like the
+// floats); a row with an infinity or NaN is left out, so that it does not undo the scale of all others.
+// 16 lanes of 8 channels a row.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_prep_kernel(AttnArgs a) {
   constexpr bool F16 = is_f16<T>;
@@ -110,7 +112,7 @@ __global__ __launch_bounds__(256) void attn_prep_kernel(AttnArgs a) {
     if constexpr (F16) {
       n = raft_row16_sum(n);
       const int k = w < nrow ? 0 : 1;
-      best[k] = max(best[k], __float_as_uint(n));
+      best[k] = max(best[k], n < INFINITY ? __float_as_uint(n) : 0u);
     }
   }
   if constexpr (F16) {

@@ -68,3 +68,27 @@ def test_plain_form_queries_without_keys(case):
 @pytest.mark.parametrize('case', range(5))
 def test_queries_without_keys(ext_ops, dt, case):
     check_unseen(DTS[dt], DEV, case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('bad', ['dout', 'v'])
+def test_other_items_keep_their_bits(ext_ops, bad):
+    """fp16: an infinity or NaN in one item makes that item's gradients useless, not coarser those of the
+    others, whose dout lies far under fp16's range without the backward's common scale: they keep the bits
+    that they have beside a finite item (the row in question is zero there, so it decides no scale)."""
+    q, k, v, do = inputs(2, 90, 1400, 1, 2, 64, torch.float16)
+    do = do * 2.0 ** -12
+    row = (do if bad == 'dout' else v)[0, 5, 0]
+    row.zero_()
+
+    def gradients():
+        leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+        return torch.autograd.grad(attention(*leaves), leaves, do)
+    clean = gradients()
+    for n, t in zip(('dq', 'dk', 'dv'), clean):
+        close(t[1:], formula(q[1:], k[1:], v[1:], do[1:]), n)
+    for value in (float('inf'), float('nan')):
+        row[3] = value
+        grads = gradients()
+        assert not all(torch.isfinite(g[0]).all() for g in grads)
+        assert all(torch.equal(a[1], b[1]) for a, b in zip(grads, clean))
