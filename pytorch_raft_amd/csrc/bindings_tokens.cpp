@@ -91,9 +91,11 @@ AttnArgs attn_args(const Tensor& q, const Tensor& k, const Tensor& v, double sca
   a.q = q.data_ptr();
   a.q_sb = stride_of(q, 0), a.q_sl = stride_of(q, 1), a.q_sh = stride_of(q, 2);
   a.k = k.data_ptr();
-  a.k_sb = stride_of(k, 0), a.k_sl = stride_of(k, 1), a.k_sh = stride_of(k, 2);
+  // (one key: a pitch past its row, so that a tile's places behind it read as zeros, not as the key again)
+  const auto pitch = [](const Tensor& t) { return t.size(1) == 1 ? t.size(3) : t.stride(1); };
+  a.k_sb = stride_of(k, 0), a.k_sl = pitch(k), a.k_sh = stride_of(k, 2);
   a.v = v.data_ptr();
-  a.v_sb = stride_of(v, 0), a.v_sl = stride_of(v, 1), a.v_sh = stride_of(v, 2);
+  a.v_sb = stride_of(v, 0), a.v_sl = pitch(v), a.v_sh = stride_of(v, 2);
   check_ints(lengths, q, B, "lengths");
   check_ints(q_offset, q, B, "q_offset");
   a.lengths = given(lengths) ? lengths->data_ptr<int>() : nullptr;

@@ -92,3 +92,27 @@ def test_other_items_keep_their_bits(ext_ops, bad):
         grads = gradients()
         assert not all(torch.isfinite(g[0]).all() for g in grads)
         assert all(torch.equal(a[1], b[1]) for a, b in zip(grads, clean))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dt', list(DTS))
+@pytest.mark.parametrize('lq', [1, 9, 140])
+def test_single_keys_hold_anything(ext_ops, dt, lq):
+    """One key: a query's output is that key's value, whatever it is, also infinite (Lk = 1, and an item
+    of one key among longer ones).  The key's probability is p = 1 + d, d from the fp32 rounding of the
+    exponent (under 2^-18 for scores of this size), and the sum l is p itself.  16-bit types: p rounds to
+    1, and v / l lies within 2^-18 of v, relative, under half a step of both types: it rounds to v.  fp32:
+    v p (1 / l) has the roundings of the product, the reciprocal (one step, 2 w) and the last product:
+    4 w, w = 2^-24."""
+    q, k, v, _ = inputs(2, lq, 1, 2, 2, 64, DTS[dt])
+    v[0, 0, 0, :3] = torch.tensor([float('inf'), float('-inf'), float('nan')])
+    out = attention(q, k, v)
+    ref = v.repeat_interleave(2, 2).expand_as(q)
+    finite = torch.isfinite(ref)
+    assert torch.equal(out[~finite].nan_to_num(7.), ref[~finite].nan_to_num(7.))
+    tol = 4 * 2.0 ** -24 if dt == 'fp32' else 0
+    assert ((out[finite] - ref[finite]).abs() <= tol * ref[finite].abs()).all()
+    long_k, long_v = (torch.full((2, 70, 2, 64), float('nan'), dtype=v.dtype, device=DEV) for _ in range(2))
+    long_k[:, :1], long_v[:, :1] = k, v
+    one = torch.ones(2, dtype=torch.int32, device=DEV)
+    assert torch.equal(attention(q, long_k, long_v, lengths=one).nan_to_num(7.), out.nan_to_num(7.))
