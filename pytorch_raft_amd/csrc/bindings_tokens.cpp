@@ -5,10 +5,12 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
+#include <initializer_list>
 #include <limits>
 #include <vector>
 
@@ -332,6 +334,13 @@ using torch::autograd::variable_list;
 
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
+// the calls below go under autograd unless an input requires a gradient: a tangent would be lost there
+void no_tangent(const char* name, std::initializer_list<Tensor> inputs) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor& t : inputs)
+    TORCH_CHECK(!t.defined() || !t._fw_grad(/*level=*/0).defined(), name, " has no forward-mode derivative");
+}
+
 void once_only(const char* name) {
   TORCH_CHECK(!at::GradMode::is_enabled(), name, " has no second derivative (create_graph)");
 }
@@ -349,6 +358,7 @@ struct AttentionNode : public torch::autograd::Function<AttentionNode> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once_only("attention");
+    no_tangent("attention's backward", {grads[0]});
     const auto s = ctx->get_saved_variables();
     const auto opt = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
     auto r = attn_bwd(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["scale"].toDouble(),
@@ -357,7 +367,7 @@ struct AttentionNode : public torch::autograd::Function<AttentionNode> {
   }
 };
 
-// q (B, Lq, H, D), k, v (B, Lk, Hkv, D), mask broadcastable to (B, H, Lq, Lk); scale 0: D ** -0.5
+// q (B, Lq, H, D), k, v (B, Lk, Hkv, D), mask broadcastable to (B, H, Lq, Lk); no scale given: D ** -0.5
 Tensor attention(const Tensor& q0, const Tensor& k0, const Tensor& v0, std::optional<double> scale0, bool causal, OptTensor mask0,
                  OptTensor lengths, OptTensor q_offset) {
   TORCH_CHECK_VALUE(q0.dim() == 4 && k0.dim() == 4 && v0.sizes() == k0.sizes(), "q must be (B, Lq, H, D), k and v (B, Lk, Hkv, D); got ",
@@ -394,6 +404,7 @@ Tensor attention(const Tensor& q0, const Tensor& k0, const Tensor& v0, std::opti
     TORCH_CHECK_VALUE(fits, "mask ", mask0->sizes(), " does not broadcast to (", B, ", ", H, ", ", Lq, ", ", Lk, ")");
     mask = mask0->expand({B, H, Lq, Lk});
   }
+  no_tangent("attention", {q0, k0, v0});
   Tensor q = q0, k = k0, v = v0;
   const int64_t pad = (8 - D % 8) % 8;
   if (pad) q = at::constant_pad_nd(q, {0, pad}), k = at::constant_pad_nd(k, {0, pad}), v = at::constant_pad_nd(v, {0, pad});
@@ -439,6 +450,7 @@ struct RmsNormNode : public torch::autograd::Function<RmsNormNode> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once_only("rms_norm");
+    for (const Tensor& t : grads) no_tangent("rms_norm's backward", {t});
     const auto s = ctx->get_saved_variables();
     const bool sum = ctx->saved_data["sum"].toBool();
     const Tensor dh = sum ? grads[1] : Tensor();
@@ -451,6 +463,7 @@ struct RmsNormNode : public torch::autograd::Function<RmsNormNode> {
 
 Tensor rms_norm(const Tensor& x, const Tensor& w, double eps) {
   rms_check(x, w, no_tensor, eps);
+  no_tangent("rms_norm", {x, w});
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w))) return RmsNormNode::apply(x, w, std::optional<Tensor>(), eps)[0];
   at::AutoDispatchBelowADInplaceOrView below;
   return rms_fwd(x.contiguous(), w.contiguous(), no_tensor, eps, false)[0];
@@ -458,6 +471,7 @@ Tensor rms_norm(const Tensor& x, const Tensor& w, double eps) {
 
 std::tuple<Tensor, Tensor> rms_norm_residual(const Tensor& x, const Tensor& w, const Tensor& residual, double eps) {
   rms_check(x, w, residual, eps);
+  no_tangent("rms_norm", {x, w, residual});
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(residual))) {
     auto r = RmsNormNode::apply(x, w, std::optional<Tensor>(residual), eps);
     return {r[0], r[1]};
@@ -472,6 +486,7 @@ std::vector<Tensor> rms_norm_int8(const Tensor& x, const Tensor& w, OptTensor re
   rms_check(x, w, residual, eps);
   TORCH_CHECK(!at::GradMode::is_enabled() || !(wants_grad(x) || wants_grad(w) || (given(residual) && wants_grad(*residual))),
               "rms_norm_int8 has no gradient: call it under torch.no_grad()");
+  no_tangent("rms_norm_int8", {x, w, given(residual) ? *residual : Tensor()});
   at::AutoDispatchBelowADInplaceOrView below;
   auto r = rms_fwd_int8(x.contiguous(), w.contiguous(), dense(residual), eps);
   if (!given(residual)) r.pop_back();
@@ -496,6 +511,7 @@ Tensor int8_linear(const Tensor& x, const Tensor& xs, const Tensor& w, const Ten
   vec(ws, {w.size(0)}, "w_scale");
   if (given(bias)) vec(*bias, {w.size(0)}, "bias");
   TORCH_CHECK_VALUE(w.device() == x.device(), "w is on ", w.device(), ", x on ", x.device());
+  no_tangent("int8_linear", {xs, ws, given(bias) ? *bias : Tensor()});
   at::AutoDispatchBelowADInplaceOrView below;
   int64_t M = 1;
   for (const int64_t n : lead) M *= n;

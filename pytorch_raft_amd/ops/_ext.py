@@ -151,6 +151,11 @@ def device_ok(t):
     return bool(t.is_cuda) or _DRY['on']
 
 
+def has_tangent(*tensors):
+    """True if one of ``tensors`` (None among them or not) carries a forward-mode derivative."""
+    return any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 # ---------------------------------------------------------------------------------------------
 # Dry run: execute the full HIP-path orchestration on CPU with every native op replaced by a
 # schema-checking stub (arguments are validated against the registered TORCH_LIBRARY schema; ops

@@ -18,8 +18,9 @@ A query that sees no key gets zeros, and zero gradients, and adds nothing to tho
 and its output's gradient may hold anything.  Where a query sees a key, an infinity or NaN in it, in what
 it sees or in its output's gradient may reach all gradients of its head.  bf16, fp16 and fp32; sums, maxima and
 accumulators are fp32, the probabilities are rounded to the inputs' type for their product with v.
-Differentiable in q, k and v (the backward recomputes the probabilities from a saved log-sum-exp; the
-same inputs give the same bits).  Head sizes up to 128 (others than multiples of 8 are padded by a
+Differentiable in q, k and v by the backward pass, once on the GPU: second and forward-mode derivatives
+raise there (the backward recomputes the probabilities from a saved log-sum-exp; the same inputs give the
+same bits).  Head sizes up to 128 (others than multiples of 8 are padded by a
 copy); less than 2^22 pairs of item and key head and less than 2^26 rows (B * H * Lq) a call.  Calls with
 at most 32 rows (H / Hkv * Lq), e.g. single tokens over a cache, run a kernel that splits the keys.
 

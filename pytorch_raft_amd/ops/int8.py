@@ -60,4 +60,6 @@ def int8_linear(x, x_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16, imp
     for name, t in (('x_scale', x_scale), ('w', w), ('w_scale', w_scale), ('bias', bias)):
         if t is not None and t.device != x.device:
             raise ValueError('%s is on %s, x on %s' % (name, t.device, x.device))
+    if _ext.has_tangent(x_scale, w_scale, bias):
+        raise RuntimeError('int8_linear has no forward-mode derivative')
     return torch_int8_linear(x, x_scale, w, w_scale, bias, out_dtype)

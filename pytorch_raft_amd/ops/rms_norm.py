@@ -3,7 +3,8 @@
 ``rms_norm(x, weight)`` -> y = x / sqrt(mean x^2 + eps) * weight.
 ``rms_norm(x, weight, residual=r)`` -> (y, h): h = x + r, rounded to the type of x (it is the stream
 that the next residual adds to), and y is the norm of h as rounded.  Differentiable in x, residual and
-weight (the encoders' fused norms, ops/encoder.py, are the per-image and per-batch counterparts).
+weight by the backward pass, once on the GPU: second and forward-mode derivatives raise there (the
+encoders' fused norms, ops/encoder.py, are the per-image and per-batch counterparts).
 
 ``rms_norm_int8(x, weight, residual=None)`` -> (q, scale, h): the same norm with an 8-bit output for
 ``int8_linear`` (ops/int8.py): q = rint(y * 127 / max|y|) int8 with one fp32 scale = max|y| / 127 per
@@ -80,4 +81,6 @@ def rms_norm_int8(x, weight, residual=None, eps=1e-6, impl='auto'):
     _check(x, weight, residual, eps)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         raise RuntimeError('rms_norm_int8 has no gradient: call it under torch.no_grad()')
+    if _ext.has_tangent(x, weight, residual):
+        raise RuntimeError('rms_norm_int8 has no forward-mode derivative')
     return torch_rms_norm_int8(x, weight, residual, eps)
