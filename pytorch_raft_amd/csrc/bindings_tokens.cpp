@@ -59,6 +59,13 @@ void check_ints(OptTensor t, const Tensor& like, int64_t n, const char* name) {
               name, " must be a contiguous int32 tensor of shape (", n, ",) on the device of q");
 }
 
+// scores are formed in fp32, in units of log 2: past its range, hidden places (-inf) would meet a factor of 0
+// or a score of 0 one of infinity, and become NaN
+bool scale_ok(double scale) {
+  const double s = scale * 1.4426950408889634;
+  return s > 0x1p-150 && s <= (double)std::numeric_limits<float>::max();
+}
+
 AttnArgs attn_args(const Tensor& q, const Tensor& k, const Tensor& v, double scale, bool causal,
                    OptTensor mask, OptTensor lengths, OptTensor q_offset) {
   TORCH_CHECK(q.is_cuda() && k.device() == q.device() && v.device() == q.device(),
@@ -72,7 +79,7 @@ AttnArgs attn_args(const Tensor& q, const Tensor& k, const Tensor& v, double sca
               "the query heads must be a multiple of the key heads");
   const int64_t B = q.size(0), Lq = q.size(1), H = q.size(2), D = q.size(3), Lk = k.size(1);
   TORCH_CHECK(D >= 8 && D <= 128 && D % 8 == 0, "head size must be a multiple of 8 up to 128, got ", D);
-  TORCH_CHECK(std::isfinite(scale) && scale > 0, "scale must be positive and finite");
+  TORCH_CHECK(scale_ok(scale), "scale must be positive and finite in fp32");
   const int64_t big = int64_t(1) << 26;
   // (grids: less than 2^24 workgroups of 256)
   TORCH_CHECK(B * H * std::max<int64_t>(Lq, 1) < big && B * k.size(2) * std::max<int64_t>(Lk, 1) < big * 16 && Lk < big * 16 &&
@@ -381,7 +388,7 @@ Tensor attention(const Tensor& q0, const Tensor& k0, const Tensor& v0, std::opti
   TORCH_CHECK_VALUE(Hkv > 0 && H > 0 && H % Hkv == 0, "the ", H, " query heads must be a multiple of the ", Hkv, " key heads");
   TORCH_CHECK_VALUE(D >= 1 && D <= 128, "head size must be 1 .. 128, got ", D);
   const double scale = scale0.has_value() ? *scale0 : 1.0 / std::sqrt((double)D);
-  TORCH_CHECK_VALUE(std::isfinite(scale) && scale > 0, "scale must be positive and finite, got ", scale);
+  TORCH_CHECK_VALUE(scale_ok(scale), "scale must be positive and finite in fp32 (2^-150 .. 2^127), got ", scale);
   const auto on = [&](const Tensor& t, const char* name) {
     TORCH_CHECK_VALUE(t.device() == q0.device(), name, " is on ", t.device(), ", q on ", q0.device());
   };

@@ -5,7 +5,7 @@ reads key head ``h // (H // Hkv)``.  A channels_last feature map (B, C, h, w) is
 a copy: ``x.permute(0, 2, 3, 1).reshape(B, h * w, heads, C // heads)``; so are the parts of one q|k|v
 projection.
 
-* ``scale``: of the scores, default ``D ** -0.5``; positive.
+* ``scale``: of the scores, default ``D ** -0.5``; positive, within fp32's range (2^-150 .. 2^127).
 * ``lengths`` (B,) int32: item b holds keys 0 .. lengths[b] - 1; what lies behind is not read.
 * ``causal``: query i of item b stands at key position ``q_offset[b] + i`` and sees the keys up to it;
   ``q_offset`` (B,) int32 defaults to ``Lk - Lq`` (the last query sees the last key).  A step over
@@ -31,6 +31,7 @@ import torch
 from . import _ext
 
 MAX_HEAD = 128
+LOG2_E = 1.4426950408889634
 
 
 def torch_attention(q, k, v, scale=None, causal=False, mask=None, lengths=None, q_offset=None):
@@ -74,8 +75,9 @@ def _check(q, k, v, scale, mask, lengths, q_offset):
         raise ValueError('head size must be 1 .. %d, got %d' % (MAX_HEAD, d))
     if not (q.dtype == k.dtype == v.dtype):
         raise TypeError('q, k and v must have one dtype, got %s, %s, %s' % (q.dtype, k.dtype, v.dtype))
-    if not 0 < scale < float('inf'):
-        raise ValueError('scale must be positive and finite, got %r' % scale)
+    # (scores are formed in fp32, in units of log 2)
+    if not 2. ** -150 < scale * LOG2_E <= torch.finfo(torch.float32).max:
+        raise ValueError('scale must be positive and finite in fp32 (2^-150 .. 2^127), got %r' % scale)
     if mask is not None:
         if mask.dtype != torch.bool:
             raise TypeError('mask must be bool (True = seen), got %s' % mask.dtype)

@@ -116,3 +116,33 @@ def test_single_keys_hold_anything(ext_ops, dt, lq):
     long_k[:, :1], long_v[:, :1] = k, v
     one = torch.ones(2, dtype=torch.int32, device=DEV)
     assert torch.equal(attention(q, long_k, long_v, lengths=one).nan_to_num(7.), out.nan_to_num(7.))
+
+
+def scale_range(dev, impl):
+    """Scores are formed in fp32, in units of log 2: a scale outside that range made every hidden place NaN
+    (0 * -inf) or every score (infinity * 0)."""
+    q, k, v, _ = inputs(1, 3, 40, 1, 1, 32, torch.float32, dev=dev)
+    mask = torch.ones(3, 40, dtype=torch.bool, device=dev)
+    mask[:, 17:] = False
+    for scale in (1e-60, 2.0 ** -151, 3e38, 1e39, 1e300, 5e-324):
+        with pytest.raises(ValueError, match='scale'):
+            attention(q, k, v, scale=scale, mask=mask, impl=impl)
+    # the smallest scales: all scores are 0 to fp32, the seen keys' mean
+    for scale in (2.0 ** -149, 1e-40, 2.0 ** -126):
+        out = attention(q, k, v, scale=scale, mask=mask, impl=impl)
+        mean = v[:, :17].double().mean(1, keepdim=True)
+        # sums of 17 terms and a division in fp32
+        assert ((out - mean).abs() <= 20 * 2.0 ** -24 * v[:, :17].double().abs().mean(1, keepdim=True)).all()
+    # large ones, where q and k are small enough
+    out = attention(q * 2.0 ** -50, k * 2.0 ** -50, v, scale=2.0 ** 100, impl=impl)
+    res = formula(q, k, v, scale=1.)
+    close(out, res, 'out')
+
+
+def test_plain_form_scales():
+    scale_range('cpu', 'torch')
+
+
+@pytest.mark.gpu
+def test_scales(ext_ops):
+    scale_range(DEV, 'hip')
