@@ -63,6 +63,7 @@ def torch_attention(q, k, v, scale=None, causal=False, mask=None, lengths=None, 
 
 
 def _check(q, k, v, scale, mask, lengths, q_offset):
+    """The operator's own checks (csrc/bindings_tokens.cpp) for the plain form; -> the scale."""
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
         raise ValueError('q must be (B, Lq, H, D), k and v (B, Lk, Hkv, D); got %s, %s, %s'
                          % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
@@ -75,6 +76,7 @@ def _check(q, k, v, scale, mask, lengths, q_offset):
         raise ValueError('head size must be 1 .. %d, got %d' % (MAX_HEAD, d))
     if not (q.dtype == k.dtype == v.dtype):
         raise TypeError('q, k and v must have one dtype, got %s, %s, %s' % (q.dtype, k.dtype, v.dtype))
+    scale = d ** -0.5 if scale is None else float(scale)
     # (scores are formed in fp32, in units of log 2)
     if not 2. ** -150 < scale * LOG2_E <= torch.finfo(torch.float32).max:
         raise ValueError('scale must be positive and finite in fp32 (2^-150 .. 2^127), got %r' % scale)
@@ -89,12 +91,12 @@ def _check(q, k, v, scale, mask, lengths, q_offset):
     for name, t in (('k', k), ('v', v), ('mask', mask), ('lengths', lengths), ('q_offset', q_offset)):
         if t is not None and t.device != q.device:
             raise ValueError('%s is on %s, q on %s' % (name, t.device, q.device))
+    return scale
 
 
 def attention(q, k, v, scale=None, causal=False, mask=None, lengths=None, q_offset=None, impl='auto'):
     if impl != 'torch' and _ext.device_ok(q) and _ext.gpu_path_enabled(required=(impl == 'hip')):
         # (checks, padding and the autograd node are the operator's own: csrc/bindings_tokens.cpp)
         return _ext.ops().attention(q, k, v, scale, causal, mask, lengths, q_offset)
-    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    _check(q, k, v, scale, mask, lengths, q_offset)
+    scale = _check(q, k, v, scale, mask, lengths, q_offset)
     return torch_attention(q, k, v, scale, causal, mask, lengths, q_offset)
