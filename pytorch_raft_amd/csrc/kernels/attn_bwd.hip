@@ -78,6 +78,7 @@ __global__ __launch_bounds__(256) void attn_prep_kernel(AttnArgs a) {
   uint32_t best[2] = {0, 0};
   for (int64_t w = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); w < nrow + nv; w += (int64_t)gridDim.x * 16) {
     float s = 0.f, n = 0.f;
+    const float l = w < nrow ? a.lse[w] : 0.f;
     if (w < nrow) {
       const int bh = (int)(w / R), row = (int)(w - (int64_t)bh * R);
       const int b = bh / a.Hkv, hk = bh - b * a.Hkv, qi = row / a.G, h = hk * a.G + row % a.G;
@@ -107,7 +108,7 @@ __global__ __launch_bounds__(256) void attn_prep_kernel(AttnArgs a) {
     }
     s = raft_row16_sum(s);
     // a row that sees no key has no part in the gradients, whatever dout holds there
-    if (w < nrow && a.lse[w] == INFINITY) s = n = 0.f;
+    if (l == INFINITY) s = n = 0.f;
     if (w < nrow && sub == 0) a.delta[w] = s;
     if constexpr (F16) {
       n = raft_row16_sum(n);

@@ -28,7 +28,6 @@ typedef __attribute__((address_space(3))) v4bf lds_v4bf;
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
 
 constexpr uint32_t kOob = 0x80000000u;  // a byte offset past every descriptor's range: reads as zeros
-constexpr float kLog2e = 1.4426950408889634f;
 
 template <typename T> struct FragOf;
 template <> struct FragOf<__bf16> { typedef v8bf type; };
@@ -188,11 +187,6 @@ struct Loader {
       const int c = chunk_of(tid, j) * 16;
       off[j] = c < dbytes ? row_of(tid, j) * pitch + c : kOob;
     }
-  }
-  // lds: wave-uniform LDS byte address of the tile + 1024 * (wave among the NTHR threads)
-  __device__ __forceinline__ void issue(rsrc_t r, uint32_t lds) const {
-#pragma unroll
-    for (int j = 0; j < PER; ++j) raft_dma16(r, lds + j * NTHR * 16, off[j]);
   }
 };
 

@@ -18,7 +18,7 @@ namespace attn_detail {
 template <typename T, int DP>
 struct FwdCfg {
   static constexpr int BK = sizeof(T) == 4 ? 32 : 64;  // keys per tile
-  static constexpr int NW = 4, NT = 256, BM = 32 * NW;
+  static constexpr int BM = 32 * 4;                    // rows of a workgroup: 32 for each of its waves
   static constexpr int TILE = BK * DP * (int)sizeof(T);
 };
 
