@@ -131,7 +131,10 @@ struct Tile {
   }
 };
 
-// eight probabilities (accumulator registers 8 t .. 8 t + 7) as a B fragment, rounded to nearest
+// eight probabilities (accumulator registers 8 t .. 8 t + 7) as a B fragment, rounded to nearest: the operand
+// type of the matrix instructions, 16 times the rate of fp32 ones.  This rounding (and that of dS) is seen in
+// the results: outputs and gradients in bf16 are off by 0.0023-0.0024 of their norm where their own rounding
+// alone makes 0.0017, in fp16 by 0.00024-0.00031 where it makes 0.0002.
 template <typename T>
 __device__ __forceinline__ typename FragOf<T>::type to_frag(const f32x16& s, int t) {
   typename FragOf<T>::type f;

@@ -5,12 +5,16 @@
 // maximum and sum are register reductions plus one half-wave exchange, rescaling the output is one
 // multiply per register, and the probabilities are the B operand of O^T = V^T P^T as they lie.
 //
-// Four waves share the K and V tiles (64 keys; 32 in fp32), double-buffered by LDS-DMA, two workgroups a
-// CU.  bf16: 8 x 7040 tokens, 2 heads of 64: 250 us, 810 TFLOP/s -- the vector unit's work on the scores
-// (about 800 cycles a tile and wave, 512 of matrix instructions) bounds it; 4 x 7040, 4 heads of 128:
-// 420 us, 970 TFLOP/s, where LDS fragment reads and matrix instructions need the same time.  Forming the
-// next tile's scores ahead (295 us for the first), 3 or 4 waves a SIMD (302, 281) and 64 rows a wave (289)
-// measured slower.
+// Four waves share the K and V tiles (64 keys; 32 in fp32), double-buffered by LDS-DMA.  Registers and LDS
+// let two workgroups stay on a CU with heads of 128, three with 96, four with 64 and five with 32 (16-bit
+// types without a mask; one to two fewer with one).
+// bf16, 8 x 7040 tokens, 2 heads of 64: 250 us, 810 TFLOP/s.  880 workgroups, all resident, three or four a
+// CU: a CU holds a wave 83 % of the time.  The vector unit is busy 59 % of all cycles (some 800 a tile and
+// wave: exponential, scaling, sum, maximum, conversion) and the matrix unit 37 % (512), and the waves spend
+// 41 % of their time ready behind another's issue.  Forming the next tile's scores ahead (295 us), 32-key
+// steps with three or four waves a SIMD (302, 281) and 64 rows a wave (289) measured slower.
+// Heads of 128: 4 x 7040, 4 heads 420 us, 970 TFLOP/s; 12 x 2852, 1 head 79 us, 630 TFLOP/s: 276 workgroups
+// of 512 that fit, so 20 CUs with two decide the time (a CU holds a wave 69 % of it).
 #include "attn_common.h"
 
 namespace attn_detail {

@@ -10,9 +10,10 @@ projection.
 * ``causal``: query i of item b stands at key position ``q_offset[b] + i`` and sees the keys up to it;
   ``q_offset`` (B,) int32 defaults to ``Lk - Lq`` (the last query sees the last key).  A step over
   caches filled to ``lengths`` passes ``q_offset = lengths - Lq``.  Without ``causal`` it changes nothing.
-* ``mask``: bool, broadcastable to (B, H, Lq, Lk), True where a query sees a key.  Keys hidden by a
-  mask that is the same for all queries and heads (a padding mask (B, 1, 1, Lk)) may hold anything; under a mask that
-  differs between queries, and under ``causal``, keys and values must be finite.
+* ``mask``: bool, broadcastable to (B, H, Lq, Lk), True where a query sees a key.  Keys hidden by a mask
+  that has one row for all queries and heads (a padding mask (B, 1, 1, Lk), or that expanded: sizes and
+  strides tell, not the values) may hold anything; under a mask with a row for each query or head, and under
+  ``causal``, keys and values must be finite also where they are hidden.
 
 A query that sees no key gets zeros, and zero gradients, and adds nothing to those of keys and values: it
 and its output's gradient may hold anything.  Where a query sees a key, an infinity or NaN in it, in what
@@ -20,9 +21,9 @@ it sees or in its output's gradient may reach all gradients of its head.  bf16, 
 accumulators are fp32, the probabilities are rounded to the inputs' type for their product with v.
 Differentiable in q, k and v by the backward pass, once on the GPU: second and forward-mode derivatives
 raise there (the backward recomputes the probabilities from a saved log-sum-exp; the same inputs give the
-same bits).  Head sizes up to 128 (others than multiples of 8 are padded by a
-copy); less than 2^22 pairs of item and key head and less than 2^26 rows (B * H * Lq) a call.  Calls with
-at most 32 rows (H / Hkv * Lq), e.g. single tokens over a cache, run a kernel that splits the keys.
+same bits).  Head sizes up to 128 (others than multiples of 8 are padded by a copy); less than 2^22 pairs
+of item and key head and less than 2^26 rows (B * H * Lq) a call.  Calls with at most 32 rows
+(H / Hkv * Lq), e.g. single tokens over a cache, run a kernel that splits the keys.
 
 The all-pairs correlation (ops/corr.py) is the same product of two feature maps without the softmax.
 """
