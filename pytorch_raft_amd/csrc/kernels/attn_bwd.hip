@@ -192,8 +192,8 @@ __device__ __forceinline__ void dkv_body(const AttnArgs& a, int bid, int grid, u
   const int key = tile * 128 + wave * 32 + (lane & 31);
   bool see = key < len;
   if constexpr (MASK == 1) see = see && a.mask[b * a.m_sb + (int64_t)min(key, a.Lk - 1) * a.m_sk] != 0;
-  // first row that sees this lane's key
-  const int row_min = a.causal ? (int)min((int64_t)(key - off) * a.G, (int64_t)INT32_MAX) : INT32_MIN;
+  // first row that sees this lane's key (a position times the heads passes 32 bits either way)
+  const int row_min = a.causal ? (int)max(min((int64_t)(key - off) * a.G, (int64_t)INT32_MAX), (int64_t)INT32_MIN) : INT32_MIN;
   // first query that sees any key of the workgroup / that sees all of them
   const int q_first = a.causal ? max(0, tile * 128 - off) : 0;
   const int q_full = a.causal ? tile * 128 + 127 - off : 0;

@@ -146,3 +146,39 @@ def test_plain_form_scales():
 @pytest.mark.gpu
 def test_scales(ext_ops):
     scale_range(DEV, 'hip')
+
+
+@pytest.mark.gpu
+def test_first_row_of_a_far_key(ext_ops):
+    """Keys far before the queries of a large group: (position - key) * heads passes 2^31.  One query at the
+    last position sees all keys that its mask leaves (some heads see none), so causal changes nothing, to
+    the bit."""
+    heads, lk = 2560, (1 << 20) + 77
+    g = torch.Generator(device=DEV).manual_seed(0)
+    mk = lambda *s: torch.randn(*s, generator=g, device=DEV).to(torch.bfloat16)  # noqa: E731
+    q, k, v, do = mk(1, 1, heads, 8), mk(1, lk, 1, 8), mk(1, lk, 1, 8), mk(1, 1, heads, 8)
+    mask = (torch.arange(heads, device=DEV) % 7 != 3)[None, :, None, None]
+    grads = []
+    for causal in (True, False):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        grads.append(torch.autograd.grad(attention(*leaves, causal=causal, mask=mask), leaves, do))
+    for n, a, b in zip(('dq', 'dk', 'dv'), *grads):
+        assert torch.equal(a, b), '%s: %d values differ' % (n, (a != b).sum())
+    assert (grads[0][2] != 0).any(-1).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('lq', [3, 90])
+def test_ends_of_lengths_and_offsets(ext_ops, lq):
+    """Lengths under 0 and past Lk, offsets at the ends of int32: clamped to what they mean."""
+    q, k, v, do = inputs(4, lq, 150, 2, 2, 32, torch.bfloat16)
+    big = 2 ** 31 - 1
+    lengths = torch.tensor([-big - 1, big, 151, 70], dtype=torch.int32, device=DEV)
+    first = torch.tensor([big, -big - 1, big, -1], dtype=torch.int32, device=DEV)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    out = attention(*leaves, causal=True, lengths=lengths, q_offset=first)
+    grads = torch.autograd.grad(out, leaves, do)
+    res = formula(q, k, v, do, causal=True, lengths=lengths.clamp(0, 150), q_offset=first.clamp(-lq, 150))
+    close(out, res, 'out')
+    for n, t in zip(('dq', 'dk', 'dv'), grads):
+        close(t, res, n)
