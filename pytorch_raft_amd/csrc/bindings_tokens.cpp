@@ -348,6 +348,15 @@ void no_tangent(const char* name, std::initializer_list<Tensor> inputs) {
     TORCH_CHECK(!t.defined() || !t._fw_grad(/*level=*/0).defined(), name, " has no forward-mode derivative");
 }
 
+// These functions call the kernels without passing the dispatcher again, so what its fallbacks would do is
+// done here: a view with a pending negation gets memory of its own, a zero tensor without any is refused.
+Tensor held(const Tensor& t) {
+  if (!t.defined()) return t;
+  TORCH_CHECK(!t._is_zerotensor(), "a zero tensor without memory (torch._efficientzerotensor): materialise it first");
+  return t.resolve_neg();
+}
+std::optional<Tensor> held(OptTensor t) { return given(t) ? std::optional<Tensor>(held(*t)) : std::nullopt; }
+
 void once_only(const char* name) {
   TORCH_CHECK(!at::GradMode::is_enabled(), name, " has no second derivative (create_graph)");
 }
@@ -366,6 +375,7 @@ struct AttentionNode : public torch::autograd::Function<AttentionNode> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once_only("attention");
     no_tangent("attention's backward", {grads[0]});
+    grads[0] = held(grads[0]);
     const auto s = ctx->get_saved_variables();
     const auto opt = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
     auto r = attn_bwd(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["scale"].toDouble(),
@@ -375,8 +385,9 @@ struct AttentionNode : public torch::autograd::Function<AttentionNode> {
 };
 
 // q (B, Lq, H, D), k, v (B, Lk, Hkv, D), mask broadcastable to (B, H, Lq, Lk); no scale given: D ** -0.5
-Tensor attention(const Tensor& q0, const Tensor& k0, const Tensor& v0, std::optional<double> scale0, bool causal, OptTensor mask0,
+Tensor attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, std::optional<double> scale0, bool causal, OptTensor mask0,
                  OptTensor lengths, OptTensor q_offset) {
+  const Tensor q0 = held(q_in), k0 = held(k_in), v0 = held(v_in);
   TORCH_CHECK_VALUE(q0.dim() == 4 && k0.dim() == 4 && v0.sizes() == k0.sizes(), "q must be (B, Lq, H, D), k and v (B, Lk, Hkv, D); got ",
                     q0.sizes(), ", ", k0.sizes(), ", ", v0.sizes());
   TORCH_CHECK_TYPE(q0.scalar_type() == k0.scalar_type() && q0.scalar_type() == v0.scalar_type(),
@@ -398,7 +409,7 @@ Tensor attention(const Tensor& q0, const Tensor& k0, const Tensor& v0, std::opti
     on(*t, name);
     TORCH_CHECK_VALUE(t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == B, name, " must be int32 of shape (", B, ",), got ",
                       t->scalar_type(), " ", t->sizes());
-    return t->contiguous();
+    return held(*t).contiguous();
   };
   const auto ln = ints(lengths, "lengths"), qo = ints(q_offset, "q_offset");
   std::optional<Tensor> mask;
@@ -409,7 +420,7 @@ Tensor attention(const Tensor& q0, const Tensor& k0, const Tensor& v0, std::opti
     bool fits = nd <= 4;
     for (int64_t d = 0; fits && d < nd; ++d) fits = mask0->size(nd - 1 - d) == 1 || mask0->size(nd - 1 - d) == want[3 - d];
     TORCH_CHECK_VALUE(fits, "mask ", mask0->sizes(), " does not broadcast to (", B, ", ", H, ", ", Lq, ", ", Lk, ")");
-    mask = mask0->expand({B, H, Lq, Lk});
+    mask = held(*mask0).expand({B, H, Lq, Lk});
   }
   no_tangent("attention", {q0, k0, v0});
   Tensor q = q0, k = k0, v = v0;
@@ -457,7 +468,10 @@ struct RmsNormNode : public torch::autograd::Function<RmsNormNode> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once_only("rms_norm");
-    for (const Tensor& t : grads) no_tangent("rms_norm's backward", {t});
+    for (Tensor& t : grads) {
+      no_tangent("rms_norm's backward", {t});
+      t = held(t);
+    }
     const auto s = ctx->get_saved_variables();
     const bool sum = ctx->saved_data["sum"].toBool();
     const Tensor dh = sum ? grads[1] : Tensor();
@@ -468,7 +482,8 @@ struct RmsNormNode : public torch::autograd::Function<RmsNormNode> {
   }
 };
 
-Tensor rms_norm(const Tensor& x, const Tensor& w, double eps) {
+Tensor rms_norm(const Tensor& x_in, const Tensor& w_in, double eps) {
+  const Tensor x = held(x_in), w = held(w_in);
   rms_check(x, w, no_tensor, eps);
   no_tangent("rms_norm", {x, w});
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w))) return RmsNormNode::apply(x, w, std::optional<Tensor>(), eps)[0];
@@ -476,7 +491,8 @@ Tensor rms_norm(const Tensor& x, const Tensor& w, double eps) {
   return rms_fwd(x.contiguous(), w.contiguous(), no_tensor, eps, false)[0];
 }
 
-std::tuple<Tensor, Tensor> rms_norm_residual(const Tensor& x, const Tensor& w, const Tensor& residual, double eps) {
+std::tuple<Tensor, Tensor> rms_norm_residual(const Tensor& x_in, const Tensor& w_in, const Tensor& residual_in, double eps) {
+  const Tensor x = held(x_in), w = held(w_in), residual = held(residual_in);
   rms_check(x, w, residual, eps);
   no_tangent("rms_norm", {x, w, residual});
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(residual))) {
@@ -489,7 +505,9 @@ std::tuple<Tensor, Tensor> rms_norm_residual(const Tensor& x, const Tensor& w, c
 }
 
 // {q, scale} or {q, scale, h}
-std::vector<Tensor> rms_norm_int8(const Tensor& x, const Tensor& w, OptTensor residual, double eps) {
+std::vector<Tensor> rms_norm_int8(const Tensor& x_in, const Tensor& w_in, OptTensor residual_in, double eps) {
+  const Tensor x = held(x_in), w = held(w_in);
+  const std::optional<Tensor> residual = held(residual_in);
   rms_check(x, w, residual, eps);
   TORCH_CHECK(!at::GradMode::is_enabled() || !(wants_grad(x) || wants_grad(w) || (given(residual) && wants_grad(*residual))),
               "rms_norm_int8 has no gradient: call it under torch.no_grad()");
@@ -501,7 +519,9 @@ std::vector<Tensor> rms_norm_int8(const Tensor& x, const Tensor& w, OptTensor re
 }
 
 // x (..., K) int8, x_scale (...), w (N, K) int8, w_scale (N)
-Tensor int8_linear(const Tensor& x, const Tensor& xs, const Tensor& w, const Tensor& ws, OptTensor bias, int64_t out_dtype) {
+Tensor int8_linear(const Tensor& x_in, const Tensor& xs_in, const Tensor& w_in, const Tensor& ws_in, OptTensor bias_in, int64_t out_dtype) {
+  const Tensor x = held(x_in), xs = held(xs_in), w = held(w_in), ws = held(ws_in);
+  const std::optional<Tensor> bias = held(bias_in);
   TORCH_CHECK_TYPE(x.scalar_type() == at::kChar && w.scalar_type() == at::kChar, "x and w must be int8, got ", x.scalar_type(), " and ",
                    w.scalar_type());
   TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(1), "x must be (..., K), w (N, K); got ", x.sizes(), ", ", w.sizes());
