@@ -17,7 +17,8 @@ _CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
 def quantize_weight(weight):
-    """(N, K) floating weight -> (int8 (N, K), fp32 scale (N,)), contiguous, symmetric per output channel; once, not per call."""
+    """(N, K) floating weight -> (int8 (N, K), fp32 scale (N,)), contiguous, symmetric per output channel; once, not
+    per call.  A row with an infinity or NaN has a scale of infinity or NaN, and its 8 bits say nothing."""
     if weight.dim() != 2 or not weight.is_floating_point():
         raise ValueError('weight must be a floating (N, K) tensor, got %s %s' % (weight.dtype, tuple(weight.shape)))
     w = weight.detach().float()

@@ -8,7 +8,8 @@ encoders' fused norms, ops/encoder.py, are the per-image and per-batch counterpa
 
 ``rms_norm_int8(x, weight, residual=None)`` -> (q, scale, h): the same norm with an 8-bit output for
 ``int8_linear`` (ops/int8.py): q = rint(y * 127 / max|y|) int8 with one fp32 scale = max|y| / 127 per
-row (both from the unrounded fp32 y; an all-zero row has scale 0; a row with a NaN has scale NaN).
+row (both from the unrounded fp32 y; an all-zero row has scale 0; a row with an infinity or NaN has a scale
+of infinity or NaN, and its 8 bits say nothing).
 h is None without a residual.  For inference: it has no gradient.
 
 x (..., C) bf16, fp16 or fp32, C up to 16384; weight (C,) fp32 or the type of x; statistics in fp32.

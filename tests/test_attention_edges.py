@@ -182,3 +182,69 @@ def test_ends_of_lengths_and_offsets(ext_ops, lq):
     close(out, res, 'out')
     for n, t in zip(('dq', 'dk', 'dv'), grads):
         close(t, res, n)
+
+
+@pytest.mark.gpu
+def test_gradients_of_long_caches(ext_ops):
+    """Keys, values and their gradients of more than 2^31 values: all are 0 but five rows at both ends, so a
+    row's sum is known: total = sum over the five of exp(s) + the number of others.  Bounds: P and dS rounded
+    once to bf16 and the result once more, 2^-8 each, scores of fp32 sums: 2^-6 of the terms' sizes."""
+    heads, d, lq = 8, 128, 33
+    lk = (1 << 31) // (heads * d) + 777
+    g = torch.Generator().manual_seed(4)
+    mk = lambda *s: torch.randn(*s, generator=g).to(torch.bfloat16)  # noqa: E731
+    rows = torch.tensor([0, 5, lk - 300, lk - 2, lk - 1])
+    other = torch.tensor([1, 1000, lk // 2, lk - 3])
+    kv, q, do = (mk(5, heads, d), mk(5, heads, d)), 0.2 * mk(lq, heads, d), mk(lq, heads, d)
+    big = [torch.zeros(1, lk, heads, d, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    for t, x in zip(big, kv):
+        t[0, rows.to(DEV)] = x.to(DEV)
+        t.requires_grad_(True)
+    qg = q[None].to(DEV).requires_grad_(True)
+    dq, dk, dv = torch.autograd.grad(attention(qg, *big, scale=0.5), (qg, *big), do[None].to(DEV))
+    q, do, k, v = (t.double().transpose(0, 1) for t in (q, do, *kv))       # (heads, rows, d)
+    s = 0.5 * q @ k.transpose(1, 2)
+    top = s.amax(-1, keepdim=True).clamp(min=0)
+    total = (s - top).exp().sum(-1, keepdim=True) + (lk - 5) * (-top).exp()
+    p, p0 = (s - top).exp() / total, (-top).exp() / total                 # of the five, of any other key
+    o = p @ v
+    dp, delta = do @ v.transpose(1, 2), (do * o).sum(-1, keepdim=True)
+    ds, ds0, size, size0 = p * (dp - delta), -p0 * delta, p * (dp.abs() + delta.abs()), p0 * delta.abs()
+    # delta's own bound: the output off by 2^-8 sum P|v|
+    more = 2.0 ** -8 * (do.abs() * (p @ v.abs())).sum(-1, keepdim=True)
+    size, size0 = size + 64 * p * more, size0 + 64 * p0 * more
+
+    def bound(got, ref, terms):
+        assert ((got.cpu().double() - ref).abs() <= 2.0 ** -6 * terms + 1e-30).all()
+    take = lambda t, at: t[0, at.to(DEV)].transpose(0, 1)  # noqa: E731
+    bound(take(dv, rows), p.transpose(1, 2) @ do, p.transpose(1, 2) @ do.abs())
+    bound(take(dv, other), (p0.transpose(1, 2) @ do).expand(-1, 4, -1), (p0.transpose(1, 2) @ do.abs()).expand(-1, 4, -1))
+    bound(take(dk, rows), 0.5 * ds.transpose(1, 2) @ q, 0.5 * size.transpose(1, 2) @ q.abs())
+    bound(take(dk, other), 0.5 * (ds0.transpose(1, 2) @ q).expand(-1, 4, -1), 0.5 * (size0.transpose(1, 2) @ q.abs()).expand(-1, 4, -1))
+    bound(dq[0].transpose(0, 1), 0.5 * ds @ k, 0.5 * size @ k.abs())
+
+
+@pytest.mark.gpu
+def test_gradients_of_many_queries(ext_ops):
+    """Queries, outputs and their gradients of more than 2^31 values: the last rows by the formula, and the
+    keys' gradients against those of the same rows in two calls, whose sums differ in order only."""
+    heads, d, lk = 8, 128, 40
+    lq = (1 << 31) // (heads * d) + 99
+    g = torch.Generator(device=DEV).manual_seed(4)
+    mk = lambda *s: torch.empty(*s, dtype=torch.bfloat16, device=DEV).normal_(generator=g)  # noqa: E731
+    q, do, k, v = mk(1, lq, heads, d), mk(1, lq, heads, d), mk(1, lk, heads, d), mk(1, lk, heads, d)
+
+    def grads(part):
+        leaves = [t.detach().requires_grad_(True) for t in (q[:, part], k, v)]
+        out = attention(*leaves)
+        return (out.detach(), *torch.autograd.grad(out, leaves, do[:, part]))
+    whole, first, last = (grads(s) for s in (slice(None), slice(0, lq // 2), slice(lq // 2, lq)))
+    res = formula(q[:, -50:], k, v, do[:, -50:])
+    close(whole[0][:, -50:], res, 'out')
+    close(whole[1][:, -50:], res, 'dq')
+    for i in (2, 3):
+        a, b, c = (t[i].double() for t in (whole, first, last))
+        # three results rounded once each, 2^-8 of their values, whose halves are no larger in norm than
+        # about the whole; the order of fp32 sums of 2^21 terms of random sign makes some 2^-24 2^10 of it.
+        # (A row read or written at a wrong place changes a gradient by about its own size.)
+        assert (a - b - c).norm() <= 2.0 ** -6 * a.norm()
