@@ -353,7 +353,7 @@ void no_tangent(const char* name, std::initializer_list<Tensor> inputs) {
 Tensor held(const Tensor& t) {
   if (!t.defined()) return t;
   TORCH_CHECK(!t._is_zerotensor(), "a zero tensor without memory (torch._efficientzerotensor): materialise it first");
-  return t.resolve_neg();
+  return t.is_neg() ? t.resolve_neg() : t;  // (resolve_neg passes the dispatcher whether it has work or not)
 }
 std::optional<Tensor> held(OptTensor t) { return given(t) ? std::optional<Tensor>(held(*t)) : std::nullopt; }
 
